@@ -39,9 +39,10 @@ extern "C" {
 typedef struct CUstream_st* srswa_stream_t; /* == cudaStream_t */
 
 /* element types */
-enum { SRSWA_F32 = 0, SRSWA_BF16 = 1, SRSWA_F16 = 2, SRSWA_F8E4M3 = 3, SRSWA_F8E5M2 = 4 };
+enum { SRSWA_F32 = 0, SRSWA_BF16 = 1, SRSWA_F16 = 2, SRSWA_F8E4M3 = 3, SRSWA_F8E5M2 = 4, SRSWA_I8 = 5 };
 /* (the fp8 codes are accepted where an entry point says so: the decode /
- * prefill attend's K/V caches) */
+ * prefill attend's K/V caches; SRSWA_I8 and SRSWA_F8E4M3 are the codes of the
+ * scaled 8-bit cache) */
 
 /* negative status codes */
 enum {
@@ -714,6 +715,121 @@ SRSWA_API int srswa_rope2d_apply(void* x, int dtype, int64_t B, int64_t S, int64
 SRSWA_API int srswa_rope2d_decode(const int64_t* new_ids, int64_t s_ids, int64_t B, int64_t page_id,
                                   int64_t* page, int64_t* tok, const int64_t* pf_cnt, int64_t s_pf,
                                   int64_t n_pg, srswa_stream_t stream);
+
+/* ------------------------------------------------- scaled 8-bit cache ----
+ * A paged K/V cache held in 8 bits with one fp32 scale per (page, KV head):
+ * element (page, pos, head, d) of K is code * k_scale[page, head], of V code *
+ * v_scale[page, head].  Codes are e4m3 or int8; both caches share the strides
+ * (features contiguous, any order of page / position / head).  Pages are named
+ * by block_table [R, W] int32; an id outside [0, P) names no page and its
+ * tokens are never read or written.  No counterpart in the reference, whose
+ * fp8 cache has no scales (attend_triton.py:545, 626).
+ *
+ * Rows (query rows of the attend, new tokens of the append) come in two forms:
+ *   cu_rows == NULL: row n belongs to request n / rows_per_req, at position
+ *     seq_lens[r] - rows_per_req + n % rows_per_req (the last rows of each
+ *     request; N = R * rows_per_req);
+ *   cu_rows [R + 1]: rows cu_rows[r] <= n < cu_rows[r + 1] belong to request r,
+ *     at position prefix_lens[r] + n - cu_rows[r] (varlen; cu_rows[R] = N). */
+typedef struct {
+  int64_t N, R, H, Hkv, D, P, W, block_size;
+  int64_t rows_per_req;
+  int64_t window;        /* attend: keys of the local window, < 0: every key up to the row's position */
+  int64_t sinks, K;      /* attend: first tokens that stay visible; selected-block slots per row */
+  float sm_scale;
+  int q_dtype, kv_dtype, out_dtype, idx_is64;
+  int64_t s_qn, s_qh;    /* attend: q; append: the new k [N, Hkv, D] (row, head) */
+  int64_t s_on, s_oh;    /* attend: out; append: the new v */
+  int64_t s_page, s_pos, s_head;
+  int64_t s_scale;       /* row stride of k_scale / v_scale [P, Hkv] */
+  int64_t s_bt;          /* row stride of block_table */
+  int64_t s_ti_h, s_ti_n, s_b_h, s_b_n;
+  int64_t nsplit;        /* attend: parts a row's keys are split into (0: chosen) */
+} srswa_cache8_desc;
+
+/* Append: quantises new tokens k, v [N, Hkv, D] (f32 / bf16 / f16; q_dtype)
+ * into the pages their positions fall in.  Per touched page and head, for K and
+ * V apart: s = the smallest power of two with max|x| <= qmax * s over the finite
+ * new elements (qmax 448 for e4m3, 127 for int8; s >= 2^-64); a page that holds
+ * earlier tokens keeps the larger of that and its scale, and if it grew the
+ * earlier codes become round(code * old / s).  New codes are round(x / s), to
+ * nearest even and saturated (infinities to the largest code; NaN stays NaN in
+ * e4m3 and is 0 in int8).  A page whose first token is new starts afresh: its
+ * old scale is not read.  No page may be shared by two requests of the call. */
+SRSWA_API int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, const void* v, void* k_cache,
+                                  void* v_cache, float* k_scale, float* v_scale, const int32_t* block_table,
+                                  const int32_t* seq_lens, const int32_t* cu_rows, const int32_t* prefix_lens,
+                                  srswa_stream_t stream);
+
+/* Attend: q [N, H, D] (bf16 / f16) over the cache.  The row at position p sees
+ * keys j <= p with j > p - window (every one if window < 0) or j < sinks, both
+ * without a bias, and the other keys j <= p of its selected blocks topk_idx
+ * [(Hkv,) N, K] (int32 / int64; ids outside [0, W) unused, a repeated id counts
+ * once) with the slot's bias (fp32, same layout, or NULL).  Softmax of
+ * sm_scale * q . k + bias over them; out [N, H, D] (out_dtype: q's type or F32)
+ * and lse_out [N, H] fp32 natural log (optional).  A row that sees nothing
+ * gives 0 and -inf.  Codes of keys that a row does not see never reach its
+ * result, whatever they hold.  workspace: srswa_cache8_attend_workspace_size
+ * bytes, 16-byte aligned (0: none); after a call with more than one part per
+ * row its content is scratch. */
+SRSWA_API size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen);
+SRSWA_API int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, const void* k_cache,
+                                  const void* v_cache, const float* k_scale, const float* v_scale,
+                                  const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_rows,
+                                  const int32_t* prefix_lens, const void* topk_idx, const float* bias, void* out,
+                                  float* lse_out, void* workspace, size_t workspace_bytes, srswa_stream_t stream);
+
+/* -------------------------------------------------- pages of a cache ----
+ * Block tables with reference counts: block_table [R, W] int32 (row stride
+ * s_bt; -1 past a request's pages), seq_lens [R] int32 (tokens), refs [P] int32
+ * = table entries that name the page (0: free).  The pages' data are any
+ * tensors indexed by page: base + page * stride_bytes, page_bytes each. */
+typedef struct {
+  void* base;
+  int64_t page_bytes, stride_bytes;
+} srswa_page_tensor;
+enum { SRSWA_MAX_PAGE_TENSORS = 16 };
+
+/* int32 scratch of the three calls below for n items. */
+SRSWA_API size_t srswa_pages_workspace_size(int64_t n, int64_t R, int64_t P);
+
+/* Gives up the pages of rows[i] (n row ids; ids outside [0, R) and repeats do
+ * nothing): counts down, entries -1, length 0. */
+SRSWA_API int srswa_pages_free(const int32_t* rows, int64_t n, int32_t* block_table, int64_t s_bt, int64_t R,
+                               int64_t W, int32_t* seq_lens, int32_t* refs, int64_t P, int64_t block_size,
+                               srswa_stream_t stream);
+
+/* Grows rows[i] to new_lens[i] tokens with the lowest free pages, rows served
+ * in order; an item is void if its row is outside [0, R) or was named before,
+ * or its length shrinks or passes W pages.  *short_out = items left as they
+ * were because the free pages ran out (each is made whole or not at all; every
+ * item counts towards the pages that the later ones find). */
+SRSWA_API int srswa_pages_extend(const int32_t* rows, const int32_t* new_lens, int64_t n, int32_t* block_table,
+                                 int64_t s_bt, int64_t R, int64_t W, int32_t* seq_lens, int32_t* refs, int64_t P,
+                                 int64_t block_size, int32_t* short_out, void* workspace, size_t workspace_bytes,
+                                 srswa_stream_t stream);
+
+/* children[i] becomes a copy of parents[i]: full pages are shared (counts up),
+ * a part-filled last page is copied, over all ntensors tensors, into the lowest
+ * free page, items served in order.  An item is void if a row is outside [0,
+ * R), the child holds tokens or was named before, or the parent is empty.
+ * *short_out = items not made because no page was free. */
+SRSWA_API int srswa_pages_fork(const int32_t* parents, const int32_t* children, int64_t n, int32_t* block_table,
+                               int64_t s_bt, int64_t R, int64_t W, int32_t* seq_lens, int32_t* refs, int64_t P,
+                               int64_t block_size, const srswa_page_tensor* tensors, int64_t ntensors,
+                               int32_t* short_out, void* workspace, size_t workspace_bytes, srswa_stream_t stream);
+
+/* With n = pages in use, the i-th page in use at or past n moves, over all
+ * tensors, to the i-th free page below n.  out_table [R, W] (row stride s_out)
+ * and out_refs [P] are block_table and refs after the move (each may be the
+ * input itself); the data left in the pages moved from stay as they were.
+ * *live_out = n.  workspace: srswa_pages_compact_workspace_size bytes. */
+SRSWA_API size_t srswa_pages_compact_workspace_size(int64_t P);
+SRSWA_API int srswa_pages_compact(const int32_t* block_table, int64_t s_bt, int64_t R, int64_t W,
+                                  const int32_t* refs, int64_t P, const srswa_page_tensor* tensors,
+                                  int64_t ntensors, int32_t* out_table, int64_t s_out, int32_t* out_refs,
+                                  int32_t* live_out, void* workspace, size_t workspace_bytes,
+                                  srswa_stream_t stream);
 
 #ifdef __cplusplus
 }

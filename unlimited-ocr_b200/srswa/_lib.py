@@ -15,7 +15,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SRSWA_LIB", os.path.join(_HERE, "libsrswa.so"))
 
-F32, BF16, F16, F8E4M3, F8E5M2 = 0, 1, 2, 3, 4
+F32, BF16, F16, F8E4M3, F8E5M2, I8 = 0, 1, 2, 3, 4, 5
 # fp8 only where an entry point accepts it (the attends' K/V caches)
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.float8_e4m3fn: F8E4M3,
            torch.float8_e5m2: F8E5M2}
@@ -61,6 +61,21 @@ class Peer(C.Structure):
     """srswa_peer: one peer-memory exchange region (device pointers)."""
     _fields_ = [("regions", vp), ("own_region", vp), ("slot_bytes", i64), ("rank", i64), ("world", i64),
                 ("counter", vp), ("tickets", vp), ("status", vp), ("ll", i64)]
+
+
+class Cache8Desc(C.Structure):
+    """srswa_cache8_desc: shapes and strides of the scaled 8-bit cache's calls."""
+    _fields_ = [(n, i64) for n in ("N", "R", "H", "Hkv", "D", "P", "W", "block_size", "rows_per_req", "window",
+                                   "sinks", "K")] + \
+               [("sm_scale", C.c_float), ("q_dtype", C.c_int), ("kv_dtype", C.c_int), ("out_dtype", C.c_int),
+                ("idx_is64", C.c_int)] + \
+               [(n, i64) for n in ("s_qn", "s_qh", "s_on", "s_oh", "s_page", "s_pos", "s_head", "s_scale", "s_bt",
+                                   "s_ti_h", "s_ti_n", "s_b_h", "s_b_n", "nsplit")]
+
+
+class PageTensor(C.Structure):
+    """srswa_page_tensor: one tensor indexed by page."""
+    _fields_ = [("base", vp), ("page_bytes", i64), ("stride_bytes", i64)]
 
 
 _SIGS = {
@@ -139,6 +154,16 @@ _SIGS = {
     "srswa_rope2d_apply": (C.c_int, [vp, C.c_int, i64, i64, i64, i64, i64, i64, i64, vp, vp, i64, vp, i64, vp,
                                      i64, i64, C.c_int, vp]),
     "srswa_rope2d_decode": (C.c_int, [vp, i64, i64, i64, vp, vp, vp, i64, i64, vp]),
+    "srswa_cache8_append": (C.c_int, [C.POINTER(Cache8Desc)] + [vp] * 11),
+    "srswa_cache8_attend_workspace_size": (C.c_size_t, [C.POINTER(Cache8Desc), C.c_int]),
+    "srswa_cache8_attend": (C.c_int, [C.POINTER(Cache8Desc)] + [vp] * 14 + [C.c_size_t, vp]),
+    "srswa_pages_workspace_size": (C.c_size_t, [i64, i64, i64]),
+    "srswa_pages_free": (C.c_int, [vp, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp]),
+    "srswa_pages_extend": (C.c_int, [vp, vp, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp, vp, C.c_size_t, vp]),
+    "srswa_pages_fork": (C.c_int, [vp, vp, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp, C.c_size_t,
+                                   vp]),
+    "srswa_pages_compact_workspace_size": (C.c_size_t, [i64]),
+    "srswa_pages_compact": (C.c_int, [vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, C.c_size_t, vp]),
 }
 
 _lib = None
