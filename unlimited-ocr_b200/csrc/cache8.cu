@@ -1,5 +1,5 @@
 // Scaled 8-bit paged cache: the append (quantise new tokens into their pages)
-// and the attend over it.
+// and the C entries of the append and the attend.
 //
 // Append.  Per (page, head), for K and V apart:
 //   s_new = 2^ceil(log2(max|x| / qmax)) over the new elements of the page,
@@ -13,7 +13,7 @@
 
 #include <cmath>
 
-#include "cache8.cuh"
+#include "cache8_attend.cuh"
 
 namespace srswa {
 
@@ -147,97 +147,6 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const App
   }
 }
 
-struct Attend8Args {
-  const void* q;
-  const uint8_t* k;
-  const uint8_t* v;
-  const float* ks;
-  const float* vs;
-  RowMap rows;
-  const int32_t* table;
-  const void* sel;
-  const float* bias;
-  void* out;
-  float* lse;
-  int64_t s_bt, W, P, BS, N, H, Hkv, D, K;
-  int64_t window, sinks;
-  int64_t s_qn, s_qh, s_on, s_oh, s_page, s_pos, s_head, s_scale;
-  int64_t s_ti_h, s_ti_n, s_b_h, s_b_n;
-  float scale_log2;
-  int q_dtype, out_dtype, kv_dtype, idx_is64;
-};
-
-constexpr int kAttend8Threads = 128;
-
-// One CTA per (row, head): its warps take the visible keys in turn, a lane
-// holds D / 32 features, the softmax runs online in the log2 domain.
-template <int D>
-__global__ void __launch_bounds__(kAttend8Threads) cache8_attend_simple_kernel(const Attend8Args a) {
-  constexpr int E = D / 32, NW = kAttend8Threads / 32;
-  __shared__ float w_m[NW], w_l[NW], w_o[NW][D];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x, h = blockIdx.y, hk = h / (a.H / a.Hkv);
-  int64_t req, p;
-  row_place(a.rows, row, req, p);
-  int64_t ls = a.window < 0 ? 0 : p - a.window + 1;
-  if (ls < 0) ls = 0;
-  const int64_t end = min(p + 1, a.W * a.BS);  // keys past the table do not exist
-  float qv[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = load_elem(a.q, row * a.s_qn + h * a.s_qh + lane * E + e, a.q_dtype) * a.scale_log2;
-    o[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  auto keys = [&](int64_t lo, int64_t hi, float b2) {
-    for (int64_t j = lo + warp; j < hi; j += NW) {
-      const int64_t page = a.table[req * a.s_bt + j / a.BS];
-      if (page < 0 || page >= a.P) continue;
-      const int64_t off = page * a.s_page + (j % a.BS) * a.s_pos + hk * a.s_head + lane * E;
-      const int64_t so = page * a.s_scale + hk;
-      float dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) dot += qv[e] * code_to_float(a.k[off + e], a.kv_dtype);
-      const float z = warp_sum(dot) * a.ks[so] + b2;
-      const float mn = fmaxf(m, z);
-      const float al = mn == -INFINITY ? 1.f : exp2f(m - mn), pr = mn == -INFINITY ? 0.f : exp2f(z - mn);
-      l = l * al + pr;
-      const float pv = pr * a.vs[so];
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * al + pv * code_to_float(a.v[off + e], a.kv_dtype);
-      m = mn;
-    }
-  };
-  if (p >= 0) {
-    keys(0, min(min(a.sinks, ls), end), 0.f);
-    keys(ls, end, 0.f);
-    const int64_t ib = hk * a.s_ti_h + row * a.s_ti_n;
-    for (int64_t s = 0; s < a.K; ++s) {
-      const int64_t blk = load_index(a.sel, ib + s, a.idx_is64);
-      if (blk < 0 || blk >= a.W) continue;
-      bool seen = false;
-      for (int64_t t = 0; t < s; ++t) seen |= load_index(a.sel, ib + t, a.idx_is64) == blk;
-      if (seen) continue;
-      const float b2 = a.bias ? a.bias[hk * a.s_b_h + row * a.s_b_n + s] * kLog2e : 0.f;
-      keys(max(blk * a.BS, a.sinks), min(min((blk + 1) * a.BS, ls), end), b2);
-    }
-  }
-  if (lane == 0) { w_m[warp] = m; w_l[warp] = l; }
-#pragma unroll
-  for (int e = 0; e < E; ++e) w_o[warp][lane * E + e] = o[e];
-  __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < NW; ++w) M = fmaxf(M, w_m[w]);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  for (int w = 0; w < NW; ++w) L += w_l[w] * exp2f(w_m[w] - Mu);
-  for (int d = tid; d < D; d += kAttend8Threads) {
-    float acc = 0.f;
-    for (int w = 0; w < NW; ++w) acc += w_o[w][d] * exp2f(w_m[w] - Mu);
-    store_elem(a.out, row * a.s_on + h * a.s_oh + d, a.out_dtype, L > 0.f ? acc / L : 0.f);
-  }
-  if (tid == 0 && a.lse) a.lse[row * a.H + h] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
-}
-
 }  // namespace srswa
 
 using namespace srswa;
@@ -305,9 +214,8 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
 }
 
 extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen) {
-  (void)d;
-  (void)varlen;
-  return 0;
+  if (!d || d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0 || d->rows_per_req <= 0) return 0;
+  return rows_plan(*d, varlen != 0).bytes;
 }
 
 extern "C" int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, const void* k_cache,
@@ -315,8 +223,6 @@ extern "C" int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, co
                                    const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_rows,
                                    const int32_t* prefix_lens, const void* topk_idx, const float* bias, void* out,
                                    float* lse_out, void* workspace, size_t workspace_bytes, srswa_stream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   SRSWA_CHECK_ARG(d, SRSWA_EINVAL);
   const int rc = check_common(d, seq_lens, cu_rows, prefix_lens);
   if (rc) return rc;
@@ -340,10 +246,9 @@ extern "C" int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, co
   a.s_page = d->s_page; a.s_pos = d->s_pos; a.s_head = d->s_head; a.s_scale = d->s_scale;
   a.s_ti_h = d->s_ti_h; a.s_ti_n = d->s_ti_n; a.s_b_h = d->s_b_h; a.s_b_n = d->s_b_n;
   a.scale_log2 = d->sm_scale * kLog2e;
-  a.q_dtype = d->q_dtype; a.out_dtype = d->out_dtype; a.kv_dtype = d->kv_dtype; a.idx_is64 = d->idx_is64;
-  const dim3 grid(static_cast<unsigned>(d->N), static_cast<unsigned>(d->H));
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (d->D == 128) cache8_attend_simple_kernel<128><<<grid, kAttend8Threads, 0, st>>>(a);
-  else cache8_attend_simple_kernel<64><<<grid, kAttend8Threads, 0, st>>>(a);
-  return srswa_last_launch_status();
+  a.q_dtype = d->q_dtype; a.out_dtype = d->out_dtype; a.idx_is64 = d->idx_is64;
+  const RowsPlan p = rows_plan(*d, cu_rows != nullptr);
+  SRSWA_CHECK_ARG(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), SRSWA_EWORKSPACE);
+  SRSWA_CHECK_ARG(aligned(workspace, 16), SRSWA_EALIGN);
+  return rows_launch(a, p, d->kv_dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
