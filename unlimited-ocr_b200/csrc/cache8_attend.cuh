@@ -25,7 +25,7 @@ struct Attend8Args {
   int q_dtype, out_dtype, idx_is64;
   // single rows
   int64_t share, ngrp;  // rows that share a pass over the keys; column groups of an item
-  int balanced;         // 1: equal parts of all chunks per CTA, 0: one CTA per item
+  int balanced;         // 1: equal parts of all units per CTA, 0: one CTA per item
   float* part_o;        // [2 per CTA][8 columns][D] unnormalised partial outputs
   float* part_ml;       // [..][8][2] their maxima (log2) and sums
   int* part_meta;       // [CTA][4] the items its two partials belong to
@@ -35,6 +35,7 @@ struct RowsPlan {
   int64_t share, ngrp, items, ctas, o_floats;
   size_t bytes;  // workspace
   bool balanced;
+  int ch;  // 16-key chunks of a unit
 };
 RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen);
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st);
