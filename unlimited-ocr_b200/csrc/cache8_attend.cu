@@ -22,10 +22,10 @@
 //
 // Work split: the units (16 or 32 keys of one page and head) of all (row group,
 // kv head) items are laid end to end and cut into equal parts, one per resident
-// CTA, so uneven lengths leave no tail; an item cut in several parts leaves
-// fp32 partials that cache8_merge_kernel joins in order.  Each warp streams its
-// units through a private cp.async ring; its page ids and scales are
-// prefetched a block of 32 slots ahead.
+// warp, so uneven lengths leave no tail and warps never wait for one another;
+// an item cut in several parts leaves fp32 partials that cache8_merge_kernel
+// joins in order.  A warp streams its units through a private cp.async ring;
+// page ids, scales and biases are prefetched a block of 32 slots ahead.
 
 #include <cmath>
 #include <type_traits>
@@ -39,6 +39,11 @@ constexpr int kRowsThreads = 128;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsRing = 16384;  // shared memory of a warp's ring at D = 128 (half of it at 64)
 constexpr int kRowsCtasPerSm = 3;
+#ifndef PREFER_CH
+#define PREFER_CH 2
+#endif
+constexpr int kPreferCh = PREFER_CH;
+constexpr int kMaxSelected = 512;
 constexpr int kCols = 8;  // queries that share a pass over the keys (columns of the MMA)
 
 // The keys a row group can see, as slots of one page each: sinks, window,
@@ -109,6 +114,12 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// 2^x to 2 ulp, subnormal results as 0 (a softmax weight under 2^-126 is one).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -135,7 +146,7 @@ __device__ __forceinline__ uint32_t v_off(int r, int c) {
 // CH: 16-key chunks of a unit, what a warp takes at a time (a divisor of a
 // page's chunks; two amortise the softmax bookkeeping and keep two independent
 // MMA chains going).
-template <int D, int KVT, int CH>
+template <int D, int KVT, int CH, bool MULTI>
 __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kernel(const Attend8Args a) {
   constexpr int CB = 16 * D;           // bytes of a chunk of K (or V)
   constexpr int SB = 2 * CH * CB;      // bytes of a stage: K of its chunks, then V
@@ -144,16 +155,13 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   constexpr int KS = D / 16;           // MMA steps of a dot product, and feature tiles of the output
   constexpr int RPI = 512 / D;         // key rows per warp copy instruction
   extern __shared__ __align__(128) uint8_t smem[];
-  int* sel_blk = reinterpret_cast<int*>(smem + kRowsWarps * ST * SB);
-  float* sel_b2 = reinterpret_cast<float*>(sel_blk + a.K);
-  __shared__ float w_m[kRowsWarps][kCols], w_l[kRowsWarps][kCols];
-  __shared__ int64_t f_part[kRowsWarps], f_off;
-  __shared__ int f_rg;
+  __shared__ int64_t f_sum[kRowsThreads + 1];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
   const int bs = static_cast<int>(a.BS), upp = bs / UK;  // units per page
-  const int G = static_cast<int>(a.H / a.Hkv), K = static_cast<int>(a.K), share = static_cast<int>(a.share);
+  const int G = static_cast<int>(a.H / a.Hkv), K = static_cast<int>(a.K);
+  const int share = MULTI ? static_cast<int>(a.share) : 1;
   const int sinks = static_cast<int>(min(a.sinks, static_cast<int64_t>(0x7fffff00)));
   const int win = a.window < 0 ? 0x7fffff00 : static_cast<int>(min(a.window, static_cast<int64_t>(0x7fffff00)));
   const uint32_t ring = smem_u32(smem) + warp * ST * SB;
@@ -164,59 +172,55 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   // One (row group, kv head, column group), units [c0, c1) of its `s.units`;
   // slot < 0: the whole item, results written out; else partial `slot`.
   auto process = [&](int64_t rg, int64_t req, const Span& s, int64_t hk, int grp, int c0, int c1, int64_t slot) {
-    const int64_t n0 = rg * a.share;
-    __syncthreads();  // the previous item's epilogue and list are done with
-    if (K) {
-      const int64_t ib = hk * a.s_ti_h + n0 * a.s_ti_n;
-      for (int i = tid; i < K; i += kRowsThreads) {
-        const int64_t b = load_index(a.sel, ib + i, a.idx_is64);
-        sel_blk[i] = b >= 0 && b < a.W ? static_cast<int>(b) : -1;
-        sel_b2[i] = a.bias ? a.bias[hk * a.s_b_h + n0 * a.s_b_n + i] * kLog2e : 0.f;
-      }
-      __syncthreads();
-      uint32_t again = 0;  // repeats of an earlier slot (K <= 4 * threads)
-      for (int i = tid, u = 0; i < K; i += kRowsThreads, ++u)
-        if (sel_blk[i] >= 0)
-          for (int j = 0; j < i; ++j) again |= static_cast<uint32_t>(sel_blk[j] == sel_blk[i]) << u;
-      __syncthreads();
-      for (int i = tid, u = 0; i < K; i += kRowsThreads, ++u)
-        if (again >> u & 1) sel_blk[i] = -1;
-      __syncthreads();
-    }
-
+    const int64_t n0 = rg * share;
     // ---- slots: lane l of (cur, nxt) holds slot base + l, base + 32 + l ----
     const int n_fix = s.n_sink + s.n_win, nslots = n_fix + K;
     struct Pages {
       int blk, page;  // page < 0: nothing to see there
-      float ks, vs;
+      float ks, vs, b2;
     };
-    auto load_pages = [&](int i) {
-      Pages r = {0, -1, 0.f, 0.f};
-      if (i < nslots) {
-        r.blk = i < s.n_sink ? i : i < n_fix ? s.b0 + i - s.n_sink : sel_blk[i - n_fix];
-        if (r.blk >= 0) {
-          const int page = a.table[req * a.s_bt + r.blk];
-          if (page >= 0 && page < a.P) {
-            r.page = page;
-            r.ks = a.ks[page * a.s_scale + hk];
-            r.vs = a.vs[page * a.s_scale + hk];
-          }
+    auto load_pages = [&](int first) {
+      const int i = first + lane, si = i - n_fix;
+      Pages r = {i < s.n_sink ? i : s.b0 + i - s.n_sink, -1, 0.f, 0.f, 0.f};
+      bool on = i < n_fix;
+      if (first + 31 >= n_fix && first < nslots) {  // selected blocks: ids in the table, each once
+        const int64_t ib = hk * a.s_ti_h + n0 * a.s_ti_n;
+        int64_t b = -1;
+        if (si >= 0 && si < K) {
+          b = load_index(a.sel, ib + si, a.idx_is64);
+          if (a.bias) r.b2 = a.bias[hk * a.s_b_h + n0 * a.s_b_n + si] * kLog2e;
+        }
+        bool once = b >= 0 && b < a.W;
+        const int upto = min(first + 31 - n_fix, K - 1);  // the last selected slot of this block
+        for (int j0 = 0; j0 <= upto; j0 += 32) {
+          const int64_t other = j0 + lane < K ? load_index(a.sel, ib + j0 + lane, a.idx_is64) : -1;
+          for (int j = 0; j < min(32, upto - j0); ++j)
+            if (__shfl_sync(0xffffffffu, other, j) == b && j0 + j < si) once = false;
+        }
+        if (si >= 0) r.blk = once ? static_cast<int>(b) : 0;
+        on = on || (si >= 0 && once);
+      }
+      if (on) {
+        const int page = a.table[req * a.s_bt + r.blk];
+        if (page >= 0 && page < a.P) {
+          r.page = page;
+          r.ks = a.ks[page * a.s_scale + hk];
+          r.vs = a.vs[page * a.s_scale + hk];
         }
       }
       return r;
     };
     int base = (c0 / upp) & ~31;
-    Pages cur = load_pages(base + lane), nxt = load_pages(base + 32 + lane);
+    Pages cur = load_pages(base), nxt = load_pages(base + 32);
     auto limits = [&](int si, int blk, int& lo, int& hi) {
       lo = si < s.n_sink ? 0 : si < n_fix ? s.ls0 : max(blk * bs, sinks);
       hi = si < s.n_sink ? s.sink_end : si < n_fix ? s.end : min(min((blk + 1) * bs, s.ls0), s.end);
     };
 
-    // units c0 + warp, + 4, + 8 ...: the producer runs ST - 1 of them ahead
-    const int mine = (c1 - c0 - warp + kRowsWarps - 1) / kRowsWarps;
-    int p_si = (c0 + warp) / upp, p_u = (c0 + warp) % upp, p_i = 0, p_stage = 0;
+    // the producer runs ST - 1 units ahead
+    int p_si = c0 / upp, p_u = c0 % upp, p_i = c0, p_stage = 0;
     auto issue = [&]() {
-      if (p_i < mine) {
+      if (p_i < c1) {
         const int rel = p_si - base;
         const int page = rel < 32 ? __shfl_sync(0xffffffffu, cur.page, rel) : __shfl_sync(0xffffffffu, nxt.page, rel - 32);
         const int blk = rel < 32 ? __shfl_sync(0xffffffffu, cur.blk, rel) : __shfl_sync(0xffffffffu, nxt.blk, rel - 32);
@@ -244,8 +248,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
             }
           }
         }
-        p_u += kRowsWarps;
-        while (p_u >= upp) { p_u -= upp; ++p_si; }
+        if (++p_u == upp) { p_u = 0; ++p_si; }
         ++p_i;
         p_stage = p_stage + 1 == ST ? 0 : p_stage + 1;
       }
@@ -329,12 +332,12 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       }
     };
 
-    int c_si = (c0 + warp) / upp, c_u = (c0 + warp) % upp, c_stage = 0;
-    for (int i = 0; i < mine; ++i) {
+    int c_si = c0 / upp, c_u = c0 % upp, c_stage = 0;
+    for (int i = c0; i < c1; ++i) {
       if (c_si - base >= 32) {
         base += 32;
         cur = nxt;
-        nxt = load_pages(base + 32 + lane);
+        nxt = load_pages(base + 32);
       }
       cp_async_wait<ST - 2>();
       __syncwarp();  // every lane's copies have landed, and every lane is done with the stage issued next
@@ -342,12 +345,12 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       const int rel = c_si - base, si = c_si;
       const int page = __shfl_sync(0xffffffffu, cur.page, rel), blk = __shfl_sync(0xffffffffu, cur.blk, rel);
       const float ks = __shfl_sync(0xffffffffu, cur.ks, rel), vs = __shfl_sync(0xffffffffu, cur.vs, rel);
+      const float b2 = __shfl_sync(0xffffffffu, cur.b2, rel);
       int lo, hi;
       limits(si, blk, lo, hi);
       const int k0 = blk * bs + c_u * UK;
       const uint32_t src = ring + c_stage * SB;
-      c_u += kRowsWarps;
-      while (c_u >= upp) { c_u -= upp; ++c_si; }
+      if (++c_u == upp) { c_u = 0; ++c_si; }
       c_stage = c_stage + 1 == ST ? 0 : c_stage + 1;
       if (page < 0 || k0 >= hi || k0 + UK <= lo) continue;
 
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
             mma16816(x[c], a0, a1, a2, a3, qf[hseg * 4 + e][0], qf[hseg * 4 + e][1]);
           }
         }
-      const float b2 = si >= n_fix ? sel_b2[si - n_fix] : 0.f, f0 = z0 * ks, f1 = z1 * ks;
+      const float f0 = z0 * ks, f1 = z1 * ks;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         x[c][0] = fmaf(x[c][0], f0, b2);
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       // it lies in [lo, hi) and, in a group of several rows, the column's own
       // row (at p0 + r) sees it.
       bool whole = k0 >= lo && k0 + UK <= hi;
-      if (share > 1) whole = whole && k0 + UK - 1 <= s.p0 && (k0 > s.p0 + share - 1 - win || k0 + UK - 1 < sinks);
+      if (MULTI) whole = whole && k0 + UK - 1 <= s.p0 && (k0 > s.p0 + share - 1 - win || k0 + UK - 1 < sinks);
       auto sees = [&](int j, int r) { return j <= s.p0 + r && (j > s.p0 + r - win || j < sinks); };
       if (!whole) {
 #pragma unroll
@@ -392,8 +395,8 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
           for (int hh = 0; hh < 2; ++hh) {
             const int j = k0 + c * 16 + krow + 8 * hh;
             const bool in = j >= lo && j < hi;
-            if (!(in && (share == 1 || sees(j, row0)))) x[c][2 * hh] = -INFINITY;
-            if (!(in && (share == 1 || sees(j, row1)))) x[c][2 * hh + 1] = -INFINITY;
+            if (!(in && (!MULTI || sees(j, row0)))) x[c][2 * hh] = -INFINITY;
+            if (!(in && (!MULTI || sees(j, row1)))) x[c][2 * hh + 1] = -INFINITY;
           }
       }
       float c0m = -INFINITY, c1m = -INFINITY;
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       const float n0m = fmaxf(m0, c0m), n1m = fmaxf(m1, c1m);
       const float u0 = n0m == -INFINITY ? 0.f : n0m, u1 = n1m == -INFINITY ? 0.f : n1m;
       if (__any_sync(0xffffffffu, n0m != m0 || n1m != m1)) {
-        const float al0 = exp2f(m0 - u0), al1 = exp2f(m1 - u1);
+        const float al0 = ex2(m0 - u0), al1 = ex2(m1 - u1);
         l0 *= al0;
         l1 *= al1;
 #pragma unroll
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       uint32_t pb[CH][2];
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const float p0 = exp2f(x[c][0] - u0), p1 = exp2f(x[c][1] - u1), p2 = exp2f(x[c][2] - u0), p3 = exp2f(x[c][3] - u1);
+        const float p0 = ex2(x[c][0] - u0), p1 = ex2(x[c][1] - u1), p2 = ex2(x[c][2] - u0), p3 = ex2(x[c][3] - u1);
         l0 += p0 + p2;
         l1 += p1 + p3;
         pb[c][0] = transpose8x8(pack_half2(p0, p1));
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       }
       uint32_t w[CH][4][D / 32];
       load_v(src + CH * CB, w);
-      if (whole || share == 1) {  // masked keys were filled with zeros
+      if (!MULTI || whole) {  // masked keys were filled with zeros
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
           float acc[2][4] = {};
@@ -472,169 +475,197 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
     }
     cp_async_wait<0>();
 
-    // ---- join the warps ----
+    __syncwarp();  // the ring is free for the next item
+
 #pragma unroll
     for (int msk = 4; msk < 32; msk <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, msk);
       l1 += __shfl_xor_sync(0xffffffffu, l1, msk);
     }
-    __syncthreads();  // the rings become the warps' outputs
-    float* wo = reinterpret_cast<float*>(smem);
-    const int ncol = min(share * G - grp * kCols, kCols);
-    if (g == 0) {
-      w_m[warp][2 * t] = m0; w_l[warp][2 * t] = l0;
-      w_m[warp][2 * t + 1] = m1; w_l[warp][2 * t + 1] = l1;
-    }
+    // this thread: columns 2 t, 2 t + 1, features g * 2 KS .. + 2 KS - 1 (MMA
+    // rows g and g + 8 of tile e hold 2 e and 2 e + 1 of them)
 #pragma unroll
-    for (int e = 0; e < KS; ++e) {
-      const int d = g * 2 * KS + 2 * e;  // MMA rows g and g + 8 of tile e: see add_pv
-      float* x = wo + (warp * kCols + 2 * t) * D + d;
-      if (2 * t < ncol) { x[0] = o[e][0]; x[1] = o[e][2]; }
-      if (2 * t + 1 < ncol) { x[D] = o[e][1]; x[D + 1] = o[e][3]; }
-    }
-    __syncthreads();
-    for (int i = tid; i < ncol * D; i += kRowsThreads) {
-      const int c = i / D, d = i % D;
-      float M = -INFINITY;
+    for (int u = 0; u < 2; ++u) {
+      const int col = 2 * t + u, gc = grp * kCols + col;
+      if (gc >= share * G) continue;
+      const float m = u ? m1 : m0, l = u ? l1 : l0;
+      float x[2 * KS];
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, w_m[w][c]);
-      const float Mu = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
-        const float f = exp2f(w_m[w][c] - Mu);
-        L += w_l[w][c] * f;
-        acc += wo[(w * kCols + c) * D + d] * f;
+      for (int e = 0; e < KS; ++e) {
+        x[2 * e] = o[e][u];
+        x[2 * e + 1] = o[e][2 + u];
       }
       if (slot < 0) {
-        const int gc = grp * kCols + c;
         const int64_t n = n0 + gc / G, h = hk * G + gc % G;
-        store_elem(a.out, n * a.s_on + h * a.s_oh + d, a.out_dtype, L > 0.f || L != L ? acc / L : 0.f);
-        if (d == 0 && a.lse) a.lse[n * a.H + h] = L > 0.f || L != L ? (M + log2f(L)) * kLn2 : -INFINITY;
+        const bool any = l > 0.f || l != l;
+#pragma unroll
+        for (int e = 0; e < 2 * KS; ++e) x[e] = any ? x[e] / l : 0.f;
+#pragma unroll
+        for (int e = 0; e < 2 * KS; e += 8) store8(a.out, n * a.s_on + h * a.s_oh + g * 2 * KS + e, a.out_dtype, x + e);
+        if (g == 0 && a.lse) a.lse[n * a.H + h] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
       } else {
-        a.part_o[(slot * kCols + c) * D + d] = acc;
-        if (d == 0) {
-          a.part_ml[(slot * kCols + c) * 2] = M;
-          a.part_ml[(slot * kCols + c) * 2 + 1] = L;
+        float4* po = reinterpret_cast<float4*>(a.part_o + (slot * kCols + col) * D + g * 2 * KS);
+#pragma unroll
+        for (int e = 0; e < 2 * KS; e += 4) po[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        if (g == 0) {
+          a.part_ml[(slot * kCols + col) * 2] = m;
+          a.part_ml[(slot * kCols + col) * 2 + 1] = l;
         }
       }
     }
   };
 
   const int64_t per_group = a.Hkv * a.ngrp;  // items of a row group
-  int64_t req, pos, stop;
-  if (!a.balanced) {  // one CTA per item
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * kRowsWarps + warp;  // this warp's part
+  const int64_t groups = a.N / share;
+  int64_t req, pos, stop, rg, off;
+  Span s;
+  if (!a.balanced) {  // one warp per item
+    rg = me / per_group;
+    if (rg >= groups) return;
+    s = group_span<CH>(a, rg, req);
     pos = 0;
-    stop = 1;
-    f_rg = static_cast<int>(blockIdx.x / per_group);
-  } else {  // this CTA's equal part of all units
-    const int64_t groups = a.N / a.share;
+    stop = s.units;
+    off = (me % per_group) * s.units;
+  } else {  // an equal part of all units
     const int64_t per = (groups + kRowsThreads - 1) / kRowsThreads;
     const int64_t g_lo = min(tid * per, groups), g_hi = min(g_lo + per, groups);
     int64_t sum = 0;
     for (int64_t i = g_lo; i < g_hi; ++i) sum += group_span<CH>(a, i, req).units;
-    sum *= per_group;
-    int64_t x = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    if (lane == 31) f_part[warp] = x;
+    f_sum[tid + 1] = sum;
+    if (tid == 0) f_sum[0] = 0;
     __syncthreads();
-    int64_t before = x - sum, total = 0;
-    for (int w = 0; w < kRowsWarps; ++w) {
-      if (w < warp) before += f_part[w];
-      total += f_part[w];
-    }
-    pos = total * blockIdx.x / gridDim.x;
-    stop = total * (blockIdx.x + 1) / gridDim.x;
-    if (pos >= before && pos < before + sum) {
-      int64_t off = pos - before, i = g_lo;
-      for (;; ++i) {
-        const int64_t n = group_span<CH>(a, i, req).units * per_group;
-        if (off < n) break;
-        off -= n;
-      }
-      f_rg = static_cast<int>(i);
-      f_off = off;
-    }
-  }
-  __syncthreads();
-  int head_item_rg = -1, head_item = 0, tail_item_rg = -1, tail_item = 0;
-  if (pos < stop) {
-    int64_t rg = f_rg;
-    Span s = group_span<CH>(a, rg, req);
-    int64_t off = a.balanced ? f_off : (blockIdx.x % per_group) * s.units;
-    if (!a.balanced) stop = s.units;
-    while (pos < stop) {
-      const int64_t it = off / s.units;
-      const int c0 = static_cast<int>(off % s.units);
-      const int c1 = static_cast<int>(min(static_cast<int64_t>(s.units), c0 + stop - pos));
-      int64_t slot = -1;
-      if (c0 > 0) {
-        slot = 2 * static_cast<int64_t>(blockIdx.x);
-        head_item_rg = static_cast<int>(rg);
-        head_item = static_cast<int>(it);
-      } else if (c1 < s.units) {
-        slot = 2 * static_cast<int64_t>(blockIdx.x) + 1;
-        tail_item_rg = static_cast<int>(rg);
-        tail_item = static_cast<int>(it);
-      }
-      process(rg, req, s, it / a.ngrp, static_cast<int>(it % a.ngrp), c0, c1, slot);
-      pos += c1 - c0;
-      off += c1 - c0;
-      if (off == s.units * per_group && pos < stop) {
-        off = 0;
-        s = group_span<CH>(a, ++rg, req);
+    if (warp == 0) {  // prefix sums of the threads' shares
+      int64_t run = 0;
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) {
+        int64_t x = f_sum[w * 32 + lane + 1];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+          if (lane >= d) x += y;
+        }
+        f_sum[w * 32 + lane + 1] = run + x;
+        run += __shfl_sync(0xffffffffu, x, 31);
       }
     }
-  } else if (tid == 0) {
-    head_item_rg = -2;  // an empty part: the item goes on behind it
+    __syncthreads();
+    const int64_t total = f_sum[kRowsThreads] * per_group, parts = static_cast<int64_t>(gridDim.x) * kRowsWarps;
+    pos = total * me / parts;
+    stop = total * (me + 1) / parts;
+    // the share, then the row group, that holds unit `pos`
+    int lo = 0, hi = kRowsThreads;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (f_sum[mid] * per_group <= pos) lo = mid;
+      else hi = mid;
+    }
+    off = pos - f_sum[lo] * per_group;
+    rg = lo * per;
+    if (pos < stop) {
+      for (;; ++rg) {
+        s = group_span<CH>(a, rg, req);
+        if (off < s.units * per_group) break;
+        off -= s.units * per_group;
+      }
+    }
   }
-  if (tid == 0 && a.balanced) {
-    int* meta = a.part_meta + 4 * static_cast<int64_t>(blockIdx.x);
-    meta[0] = head_item_rg; meta[1] = head_item; meta[2] = tail_item_rg; meta[3] = tail_item;
+  int head_rg = pos < stop ? -1 : -2;  // -2, an empty part: an item may go on behind it
+  int head_item = 0, tail_rg = -1, tail_item = 0;
+  while (pos < stop) {
+    const int64_t it = off / s.units;
+    const int c0 = static_cast<int>(off % s.units);
+    const int c1 = static_cast<int>(min(static_cast<int64_t>(s.units), c0 + stop - pos));
+    int64_t slot = -1;
+    if (c0 > 0) {
+      slot = 2 * me;
+      head_rg = static_cast<int>(rg);
+      head_item = static_cast<int>(it);
+    } else if (c1 < s.units) {
+      slot = 2 * me + 1;
+      tail_rg = static_cast<int>(rg);
+      tail_item = static_cast<int>(it);
+    }
+    process(rg, req, s, it / a.ngrp, static_cast<int>(it % a.ngrp), c0, c1, slot);
+    pos += c1 - c0;
+    off += c1 - c0;
+    if (off == s.units * per_group && pos < stop) {
+      off = 0;
+      s = group_span<CH>(a, ++rg, req);
+    }
   }
+  if (lane == 0 && a.balanced) reinterpret_cast<int4*>(a.part_meta)[me] = make_int4(head_rg, head_item, tail_rg, tail_item);
 }
 
-// Joins the parts of the item that CTA blockIdx.x began and did not finish, in
-// the order of the parts.
+// Joins the parts of one column (blockIdx.y) of the item that part blockIdx.x
+// began and did not finish, in their order: the weights first, then the four
+// warps add every fourth part's features, then the four sums are added.
 template <int D>
-__global__ void __launch_bounds__(256) cache8_merge_kernel(const Attend8Args a, int ncta) {
+__global__ void __launch_bounds__(128) cache8_merge_kernel(const Attend8Args a, int parts) {
+  constexpr int V = D / 32;  // features of a lane
+  __shared__ float wt[128], red[4][D], top[4];
   pdl_wait();
-  const int c = blockIdx.x;
-  const int rg = a.part_meta[4 * c + 2], it = a.part_meta[4 * c + 3];
+  const int c = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int4* meta = reinterpret_cast<const int4*>(a.part_meta);
+  const int rg = meta[c].z, it = meta[c].w;
   if (rg < 0) return;
-  int last = c;  // last part of the item
-  for (int j = c + 1; j < ncta; ++j) {
-    const int r = a.part_meta[4 * j], i = a.part_meta[4 * j + 1];
-    if (r == -2) continue;
-    if (r != rg || i != it) break;
-    last = j;
-    if (a.part_meta[4 * j + 2] >= 0) break;  // this CTA went on to another item
-  }
   const int64_t hk = it / a.ngrp;
-  const int grp = static_cast<int>(it % a.ngrp), G = static_cast<int>(a.H / a.Hkv);
-  const int ncol = min(static_cast<int>(a.share) * G - grp * kCols, kCols);
-  for (int i = threadIdx.x; i < ncol * D; i += blockDim.x) {
-    const int col = i / D, d = i % D;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int j = c; j <= last; ++j) {
-      if (j > c && a.part_meta[4 * j] == -2) continue;
-      const int64_t slot = (j == c ? 2 * static_cast<int64_t>(j) + 1 : 2 * static_cast<int64_t>(j)) * kCols + col;
-      const float m = a.part_ml[slot * 2], l = a.part_ml[slot * 2 + 1];
-      const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.f : mn;
-      const float fo = exp2f(M - mu), fn = exp2f(m - mu);
-      L = L * fo + l * fn;
-      acc = acc * fo + a.part_o[slot * D + d] * fn;
-      M = mn;
+  const int grp = static_cast<int>(it % a.ngrp), G = static_cast<int>(a.H / a.Hkv), gc = grp * kCols + col;
+  if (gc >= a.share * G) return;
+  // the parts behind it that go on with the item: a run, with empty parts in it
+  int end = c + 1;
+  for (;; end += 32) {
+    const int j = end + lane;
+    const int4 x = j < parts ? meta[j] : make_int4(-1, 0, 0, 0);
+    const unsigned stop = __ballot_sync(0xffffffffu, !(x.x == -2 || (x.x == rg && x.y == it)));
+    if (stop) {
+      end += __ffs(stop) - 1;
+      break;
     }
-    const int gc = grp * kCols + col;
-    const int64_t n = static_cast<int64_t>(rg) * a.share + gc / G, h = hk * G + gc % G;
-    store_elem(a.out, n * a.s_on + h * a.s_oh + d, a.out_dtype, L > 0.f || L != L ? acc / L : 0.f);
-    if (d == 0 && a.lse) a.lse[n * a.H + h] = L > 0.f || L != L ? (M + log2f(L)) * kLn2 : -INFINITY;
   }
+  float M = -INFINITY, L = 0.f, acc[V] = {};
+  for (int j0 = c; j0 < end; j0 += 128) {
+    const int j = j0 + tid;
+    const bool on = j < end && (j == c || meta[j].x != -2);
+    const int64_t at = (j == c ? 2 * static_cast<int64_t>(j) + 1 : 2 * static_cast<int64_t>(j)) * kCols + col;
+    const float m = on ? a.part_ml[at * 2] : -INFINITY, l = on ? a.part_ml[at * 2 + 1] : 0.f;
+    const float wm = warp_max(m);
+    __syncthreads();  // the previous round's weights are used up
+    if (lane == 0) top[warp] = wm;
+    __syncthreads();
+    const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), M), mu = mn == -INFINITY ? 0.f : mn;
+    const float old = exp2f(M - mu), f = on ? exp2f(m - mu) : -1.f;  // -1: nothing was written there
+    wt[tid] = f;
+    __syncthreads();
+    L = L * old + warp_sum(on ? l * f : 0.f);  // this warp's 32 parts of each round
+    M = mn;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= old;
+    const int n = min(128, end - j0);
+#pragma unroll 4
+    for (int i = warp; i < n; i += 4) {
+      const float w = wt[i];
+      if (w >= 0.f || w != w) {
+        const int64_t part = j0 + i;
+        const float* x = a.part_o + ((part == c ? 2 * part + 1 : 2 * part) * kCols + col) * D + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) red[warp][lane * V + e] = acc[e];
+  __syncthreads();
+  if (lane == 0) top[warp] = L;
+  __syncthreads();
+  L = (top[0] + top[1]) + (top[2] + top[3]);
+  const int64_t n = static_cast<int64_t>(rg) * a.share + gc / G, h = hk * G + gc % G;
+  const bool any = L > 0.f || L != L;
+  if (tid < D) {
+    const float x = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+    store_elem(a.out, n * a.s_on + h * a.s_oh + tid, a.out_dtype, any ? x / L : 0.f);
+  }
+  if (tid == 0 && a.lse) a.lse[n * a.H + h] = any ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
 static int sm_count() {
@@ -657,7 +688,7 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   const int64_t groups = d.N / p.share;
   p.items = groups * d.Hkv * p.ngrp;
   // the most units an item can have
-  p.ch = d.block_size % 32 == 0 ? 2 : 1;
+  p.ch = d.block_size % 32 == 0 ? kPreferCh : 1;
   const int64_t upp = d.block_size / (16 * p.ch);
   int64_t blocks = d.W;
   if (d.window >= 0) {
@@ -666,47 +697,53 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
     blocks = win < d.W && snk < d.W && win + snk < d.W ? win + snk : d.W;
   }
   const int64_t most = (blocks + d.K) * upp;
-  const int64_t slots = static_cast<int64_t>(sm_count()) * kRowsCtasPerSm;
+  const int64_t slots = static_cast<int64_t>(sm_count()) * kRowsCtasPerSm * kRowsWarps;
+  int64_t parts;
   if (d.nsplit > 0) {
     p.balanced = d.nsplit > 1;
-    p.ctas = d.nsplit * p.items;
-  } else if (most <= 4 * kRowsWarps || groups > 2048 || p.items > 16 * slots) {
-    // short items (a join would cost more than it saves), or so many that their
-    // uneven ends do not show: one CTA each
+    parts = d.nsplit * p.items;
+  } else if (most <= 2 || groups > 2048 || p.items > 16 * slots) {
+    // items that a warp is through with at once, or so many that their uneven
+    // ends do not show: one warp each, no join
     p.balanced = false;
-    p.ctas = p.items;
+    parts = p.items;
   } else {
     p.balanced = true;
-    const int64_t enough = (p.items * most + kRowsWarps - 1) / kRowsWarps;
-    p.ctas = enough < slots ? enough : slots;
+    const int64_t enough = (p.items * most + 1) / 2;  // two units each at least
+    parts = enough < slots ? enough : slots;
   }
+  p.ctas = (parts + kRowsWarps - 1) / kRowsWarps;
   if (p.balanced) {
-    const int64_t f = p.ctas * 2 * kCols;
+    parts = p.ctas * kRowsWarps;
+    const int64_t f = parts * 2 * kCols;
     p.o_floats = f * d.D;
-    p.bytes = static_cast<size_t>(p.o_floats + f * 2 + p.ctas * 4) * 4;
+    p.bytes = static_cast<size_t>(p.o_floats + f * 2 + parts * 4) * 4;
   }
   return p;
 }
 
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st) {
-  if (a.K > 4 * kRowsThreads || p.ctas >= (1ll << 30)) return SRSWA_ETOOLARGE;
+  if (a.K > kMaxSelected || p.ctas >= (1ll << 28)) return SRSWA_ETOOLARGE;
   a.share = p.share;
   a.ngrp = p.ngrp;
   a.balanced = p.balanced ? 1 : 0;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + p.o_floats;
-  a.part_meta = reinterpret_cast<int*>(a.part_ml + p.ctas * 2 * kCols * 2);
+  const int64_t parts = p.ctas * kRowsWarps;
+  a.part_meta = reinterpret_cast<int*>(a.part_ml + parts * 2 * kCols * 2);
   const int ring = kRowsWarps * kRowsRing * static_cast<int>(a.D) / 128;
   auto go = [&](auto kern) -> int {
-    static_assert(kCols * 128 * 4 <= kRowsRing, "a warp's outputs fit its ring");
-    SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        ring + 4 * kRowsThreads * 8));
-    kern<<<static_cast<unsigned>(p.ctas), kRowsThreads, ring + static_cast<int>(a.K) * 8, st>>>(a);
+    SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    kern<<<static_cast<unsigned>(p.ctas), kRowsThreads, ring, st>>>(a);
     return srswa_last_launch_status();
   };
   auto by_type = [&](auto d_, auto ch_) -> int {
     constexpr int D = decltype(d_)::value, CH = decltype(ch_)::value;
-    return kv_dtype == SRSWA_I8 ? go(cache8_rows_kernel<D, SRSWA_I8, CH>) : go(cache8_rows_kernel<D, SRSWA_F8E4M3, CH>);
+    if (p.share > 1)
+      return kv_dtype == SRSWA_I8 ? go(cache8_rows_kernel<D, SRSWA_I8, CH, true>)
+                                  : go(cache8_rows_kernel<D, SRSWA_F8E4M3, CH, true>);
+    return kv_dtype == SRSWA_I8 ? go(cache8_rows_kernel<D, SRSWA_I8, CH, false>)
+                                : go(cache8_rows_kernel<D, SRSWA_F8E4M3, CH, false>);
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
@@ -716,16 +753,16 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
                             : (p.ch == 2 ? by_type(D64(), Two()) : by_type(D64(), One()));
   if (rc || !p.balanced) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(parts), static_cast<unsigned>(p.share * (a.H / a.Hkv) < kCols ? p.share * (a.H / a.Hkv) : kCols), 1);
+  cfg.blockDim = dim3(128, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = a.D == 128 ? cudaLaunchKernelEx(&cfg, cache8_merge_kernel<128>, a, static_cast<int>(p.ctas))
-                                   : cudaLaunchKernelEx(&cfg, cache8_merge_kernel<64>, a, static_cast<int>(p.ctas));
+  const cudaError_t e = a.D == 128 ? cudaLaunchKernelEx(&cfg, cache8_merge_kernel<128>, a, static_cast<int>(parts))
+                                   : cudaLaunchKernelEx(&cfg, cache8_merge_kernel<64>, a, static_cast<int>(parts));
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
 

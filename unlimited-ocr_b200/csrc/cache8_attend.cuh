@@ -25,10 +25,10 @@ struct Attend8Args {
   int q_dtype, out_dtype, idx_is64;
   // single rows
   int64_t share, ngrp;  // rows that share a pass over the keys; column groups of an item
-  int balanced;         // 1: equal parts of all units per CTA, 0: one CTA per item
-  float* part_o;        // [2 per CTA][8 columns][D] unnormalised partial outputs
+  int balanced;         // 1: equal parts of all units per warp, 0: one warp per item
+  float* part_o;        // [2 per part][8 columns][D] unnormalised partial outputs
   float* part_ml;       // [..][8][2] their maxima (log2) and sums
-  int* part_meta;       // [CTA][4] the items its two partials belong to
+  int* part_meta;       // [part][4] the items its two partials belong to (row group, item, twice)
 };
 
 struct RowsPlan {
