@@ -722,6 +722,20 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   return p;
 }
 
+template <int D, int KVT, int CH, bool MULTI>
+static int rows_start(const Attend8Args& a, unsigned ctas, int ring, cudaStream_t st) {
+  auto kern = cache8_rows_kernel<D, KVT, CH, MULTI>;
+  static bool allowed[64] = {};  // per device: the shared memory has been asked for
+  int dev = 0;
+  SRSWA_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !allowed[dev]) {
+    SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    if (dev < 64) allowed[dev] = true;
+  }
+  kern<<<ctas, kRowsThreads, ring, st>>>(a);
+  return srswa_last_launch_status();
+}
+
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st) {
   if (a.K > kMaxSelected || p.ctas >= (1ll << 28)) return SRSWA_ETOOLARGE;
   a.share = p.share;
@@ -732,18 +746,14 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   const int64_t parts = p.ctas * kRowsWarps;
   a.part_meta = reinterpret_cast<int*>(a.part_ml + parts * 2 * kCols * 2);
   const int ring = kRowsWarps * kRowsRing * static_cast<int>(a.D) / 128;
-  auto go = [&](auto kern) -> int {
-    SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
-    kern<<<static_cast<unsigned>(p.ctas), kRowsThreads, ring, st>>>(a);
-    return srswa_last_launch_status();
-  };
+  const unsigned ctas = static_cast<unsigned>(p.ctas);
   auto by_type = [&](auto d_, auto ch_) -> int {
     constexpr int D = decltype(d_)::value, CH = decltype(ch_)::value;
     if (p.share > 1)
-      return kv_dtype == SRSWA_I8 ? go(cache8_rows_kernel<D, SRSWA_I8, CH, true>)
-                                  : go(cache8_rows_kernel<D, SRSWA_F8E4M3, CH, true>);
-    return kv_dtype == SRSWA_I8 ? go(cache8_rows_kernel<D, SRSWA_I8, CH, false>)
-                                : go(cache8_rows_kernel<D, SRSWA_F8E4M3, CH, false>);
+      return kv_dtype == SRSWA_I8 ? rows_start<D, SRSWA_I8, CH, true>(a, ctas, ring, st)
+                                  : rows_start<D, SRSWA_F8E4M3, CH, true>(a, ctas, ring, st);
+    return kv_dtype == SRSWA_I8 ? rows_start<D, SRSWA_I8, CH, false>(a, ctas, ring, st)
+                                : rows_start<D, SRSWA_F8E4M3, CH, false>(a, ctas, ring, st);
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;

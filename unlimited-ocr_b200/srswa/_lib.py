@@ -154,9 +154,9 @@ _SIGS = {
     "srswa_rope2d_apply": (C.c_int, [vp, C.c_int, i64, i64, i64, i64, i64, i64, i64, vp, vp, i64, vp, i64, vp,
                                      i64, i64, C.c_int, vp]),
     "srswa_rope2d_decode": (C.c_int, [vp, i64, i64, i64, vp, vp, vp, i64, i64, vp]),
-    "srswa_cache8_append": (C.c_int, [C.POINTER(Cache8Desc)] + [vp] * 11),
-    "srswa_cache8_attend_workspace_size": (C.c_size_t, [C.POINTER(Cache8Desc), C.c_int]),
-    "srswa_cache8_attend": (C.c_int, [C.POINTER(Cache8Desc)] + [vp] * 14 + [C.c_size_t, vp]),
+    "srswa_cache8_append": (C.c_int, [vp] * 12),
+    "srswa_cache8_attend_workspace_size": (C.c_size_t, [vp, C.c_int]),
+    "srswa_cache8_attend": (C.c_int, [vp] * 15 + [C.c_size_t, vp]),
     "srswa_pages_workspace_size": (C.c_size_t, [i64, i64, i64]),
     "srswa_pages_free": (C.c_int, [vp, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp]),
     "srswa_pages_extend": (C.c_int, [vp, vp, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp, vp, C.c_size_t, vp]),
