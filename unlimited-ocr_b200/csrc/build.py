@@ -22,7 +22,7 @@ OUT = os.path.join(PKG, "srswa", "libsrswa.so")
 BUILD = os.path.join(HERE, "_build")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["api.cu", "route.cu", "attend.cu", "gather.cu", "gather_tc.cu", "page_gate.cu", "peer.cu", "kl.cu",
-           "cache8.cu", "cache8_attend.cu", "pages.cu"]
+           "cache8.cu", "cache8_attend.cu", "cache8_prompt.cu", "pages.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

@@ -215,6 +215,7 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
 
 extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen) {
   if (!d || d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0 || d->rows_per_req <= 0) return 0;
+  if (prompt_applies(*d, varlen != 0)) return 16;  // the status word
   return rows_plan(*d, varlen != 0).bytes;
 }
 
@@ -247,8 +248,14 @@ extern "C" int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, co
   a.s_ti_h = d->s_ti_h; a.s_ti_n = d->s_ti_n; a.s_b_h = d->s_b_h; a.s_b_n = d->s_b_n;
   a.scale_log2 = d->sm_scale * kLog2e;
   a.q_dtype = d->q_dtype; a.out_dtype = d->out_dtype; a.idx_is64 = d->idx_is64;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (prompt_applies(*d, cu_rows != nullptr)) {
+    SRSWA_CHECK_ARG(workspace && workspace_bytes >= 16, SRSWA_EWORKSPACE);
+    SRSWA_CHECK_ARG(aligned(workspace, 16), SRSWA_EALIGN);
+    return prompt_launch(a, d->kv_dtype, static_cast<int*>(workspace), st);
+  }
   const RowsPlan p = rows_plan(*d, cu_rows != nullptr);
   SRSWA_CHECK_ARG(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), SRSWA_EWORKSPACE);
   SRSWA_CHECK_ARG(aligned(workspace, 16), SRSWA_EALIGN);
-  return rows_launch(a, p, d->kv_dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+  return rows_launch(a, p, d->kv_dtype, workspace, st);
 }

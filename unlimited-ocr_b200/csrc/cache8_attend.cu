@@ -73,31 +73,6 @@ __device__ __forceinline__ Span group_span(const Attend8Args& a, int64_t rg, int
   return s;
 }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
-
-// Four codes -> f16 pairs (e0, e1) and (e2, e3), exactly.
-template <int KVT>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (KVT == SRSWA_I8) {  // 1024 + (c + 128) as an f16 bit pattern, minus 1152
-    const uint32_t x = w ^ 0x80808080u;
-    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
-    const uint32_t a = prmt(x, 0x64646464u, 0x4140u), b = prmt(x, 0x64646464u, 0x4342u);
-    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-    const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&ha);
-    hi = *reinterpret_cast<const uint32_t*>(&hb);
-  } else {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-  }
-}
-
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -108,16 +83,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// 2^x to 2 ulp, subnormal results as 0 (a softmax weight under 2^-126 is one).
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
