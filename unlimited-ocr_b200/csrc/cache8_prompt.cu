@@ -34,6 +34,7 @@
 // a row that does see one turns to NaN.
 
 #include <cmath>
+#include <type_traits>
 
 #include "cache8_attend.cuh"
 #include "tc.cuh"
@@ -80,6 +81,11 @@ __device__ __noinline__ bool pr_wait_slow(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
   const uint32_t a = smem_u32(bar);
   return mbar_try_wait(a, parity) || pr_wait_slow(a, parity, abort_flag, code);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&w)[16]) {
   asm volatile(
@@ -297,42 +303,49 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       if (!ok) break;
       tc_fence_after();
       check_nan();
-      float f[8];
-      {
-        const float4 x = *reinterpret_cast<const float4*>(&g_ks[ri][0]), y = *reinterpret_cast<const float4*>(&g_ks[ri][4]);
-        f[0] = x.x * rowf; f[1] = x.y * rowf; f[2] = x.z * rowf; f[3] = x.w * rowf;
-        f[4] = y.x * rowf; f[5] = y.y * rowf; f[6] = y.z * rowf; f[7] = y.w * rowf;
-      }
       const uint32_t on = g_on[ri];
       const bool whole = T.whole(s, i) && on == 0xffu;
-      uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-      if (!whole) {
+      // keys kb .. kb + 31 that this row sees
+      auto sees = [&](int c) {
+        const int kb = k0 + 32 * c, up = min(p + 1, T.key_end(i)) - kb;
+        return (bit_range(max(p - T.win + 1, 0) - kb, up) | bit_range(0, min(T.sinks - kb, up))) &
+               ((on >> (2 * c) & 1 ? 0xffffu : 0u) | (on >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
+      };
+      auto group_max = [&](const float* v, int grp) {  // of 16 raw scores, in z units
+        float x = max3(v[0], v[1], v[2]), y = max3(v[3], v[4], v[5]);
+        x = max3(x, v[6], v[7]);
+        y = max3(y, v[8], v[9]);
+        x = max3(x, v[10], v[11]);
+        y = max3(y, v[12], v[13]);
+        x = max3(x, v[14], v[15]);
+        x = fmaxf(x, y);
+        return x == -INFINITY ? x : x * (g_ks[ri][grp] * rowf);
+      };
+      // the row's largest score.  WHOLE is compile-time: a run-time test would be
+      // turned into selects on every score
+      auto largest = [&](auto whole_) {
+        constexpr bool WHOLE = decltype(whole_)::value;
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          float v[32], w[32];
+          tmem_ld32(tm_s + 32 * c, v);
+          tmem_ld32(tm_s + 32 * c + 32, w);
+          tmem_wait_ld();
+          if (!WHOLE) {
+            const uint32_t va = sees(c), vb = sees(c + 1);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int kb = k0 + 32 * c, up = min(p + 1, T.key_end(i)) - kb;
-          vis[c] = (bit_range(max(p - T.win + 1, 0) - kb, up) | bit_range(0, min(T.sinks - kb, up))) &
-                   ((on >> (2 * c) & 1 ? 0xffffu : 0u) | (on >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
+            for (int e = 0; e < 32; ++e) {
+              v[e] = va >> e & 1 ? v[e] : -INFINITY;
+              w[e] = vb >> e & 1 ? w[e] : -INFINITY;
+            }
+          }
+          mx = fmaxf(mx, max3(group_max(v, 2 * c), group_max(v + 16, 2 * c + 1), group_max(w, 2 * c + 2)));
+          mx = fmaxf(mx, group_max(w + 16, 2 * c + 3));
         }
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        tmem_ld32(tm_s + 32 * c, v);
-        tmem_wait_ld();
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = vis[c] >> e & 1 ? v[e] : -INFINITY;
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float x[4] = {v[16 * g], v[16 * g + 1], v[16 * g + 2], v[16 * g + 3]};
-#pragma unroll
-          for (int e = 4; e < 16; ++e) x[e & 3] = fmaxf(x[e & 3], v[16 * g + e]);
-          const float gm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          mx = fmaxf(mx, whole || gm != -INFINITY ? gm * f[2 * c + g] : -INFINITY);
-        }
-      }
+        return mx;
+      };
+      const float mx = whole ? largest(std::true_type()) : largest(std::false_type());
       const float top = g_top[ri];
       // the same in every thread
       const bool move_v = on && (top > lref || (top < lref - 10.f && top > lref - 60.f));
@@ -342,7 +355,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         const float ln = move_v ? top : lref;
         const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn), alpha_o = alpha * exp2f(lref - ln);
         if (cnt > 0) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             float v[32];
             tmem_ld32(tm_o + 32 * c, v);
@@ -357,40 +370,59 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         m = mn;
         lref = ln;
       }
-      const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        tmem_ld32(tm_s + 32 * c, v);
-        tmem_wait_ld();
+      const float base = kPrShift - (m == -INFINITY ? 0.f : m);
+      // weights of 32 keys -> f16 pairs over their scores' first 16 columns
+      auto weights = [&](auto whole_, float (&v)[32], int c) {
+        constexpr bool WHOLE = decltype(whole_)::value;
+        const uint32_t vis = WHOLE ? 0xffffffffu : sees(c);
         uint32_t w[16];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          // (under 2^-64 of vref a value adds nothing to O; its weight still counts in l)
-          float lv = g_lv[ri][2 * c + g] - lref;
+          const int grp = 2 * c + g;
+          float lv = g_lv[ri][grp] - lref;  // the value scale, relative to vref
           if (lv < -64.f) lv = -64.f;
-          const float add = lv + (kPrShift - mu);
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float f = g_ks[ri][grp] * rowf, add = lv + base;
+          const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x = fmaf(v[16 * g + e], f[2 * c + g], add);
-            if (!whole) x = vis[c] >> (16 * g + e) & 1 ? x : -INFINITY;
-            v[16 * g + e] = ex2(x);
-            sum[e & 3] += v[16 * g + e];
+          for (int e = 0; e < 8; ++e) {
+            const int k = 16 * g + 2 * e;
+            float2 x = __ffma2_rn(make_float2(v[k], v[k + 1]), f2, add2);
+            if (!WHOLE) {
+              x.x = vis >> k & 1 ? x.x : -INFINITY;
+              x.y = vis >> (k + 1) & 1 ? x.y : -INFINITY;
+            }
+            x = make_float2(ex2(x.x), ex2(x.y));
+            sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+            w[8 * g + e] = pack_half2(x.x, x.y);
           }
-          const float gs = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          if (whole || (vis[c] >> (16 * g) & 0xffffu)) l = fmaf(gs, ex2(-lv), l);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[8 * g + e] = pack_half2(v[16 * g + 2 * e], v[16 * g + 2 * e + 1]);
+          sum[0] = __fadd2_rn(sum[0], sum[1]);
+          if (WHOLE || (vis >> (16 * g) & 0xffffu)) l = fmaf(sum[0].x + sum[0].y, ex2(-lv), l);
         }
         tmem_st16u(tm_s + 16 * c, w);
-      }
+      };
+      auto all_weights = [&](auto whole_) {
+        float v[32], w[32];
+        tmem_ld32(tm_s, v);
+        tmem_wait_ld();
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld32(tm_s + 32 * c + 32, w);
+          weights(whole_, v, c);
+          tmem_wait_ld();
+          if (c == 0) tmem_ld32(tm_s + 64, v);
+          weights(whole_, w, c + 1);
+          if (c == 0) tmem_wait_ld();
+        }
+      };
+      if (whole) all_weights(std::true_type());
+      else all_weights(std::false_type());
       tmem_wait_st();
       tc_fence_before();
       pr_arrive(&p_full[s]);
       if (KVT != SRSWA_I8 && !whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) seen[c] = vis[c];
+        for (int c = 0; c < 4; ++c) seen[c] = sees(c);
         seen_at = i & 15;
       }
       ++cnt;
@@ -424,7 +456,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
     constexpr int UPK = D / 16;            // 16-byte units of a key's codes
     constexpr int RPP = 128 / UPK;         // keys per pass of the 128 threads
     constexpr int NP = kPrKeys / RPP;      // passes per tile
-    const int c = tid - kPrConv * 32, u = c % UPK, kr = c / UPK;
+    // unit and key of this thread in a pass.  8 lanes store 16 bytes each at once:
+    // two neighbouring keys, so that the swizzle spreads them over all banks
+    const int c = tid - kPrConv * 32;
+    const int u = D == 128 ? (c & 3) + (c >> 1 & 4) : c % UPK;
+    const int kr = D == 128 ? (c >> 2 & 1) + (c >> 3 & ~1) : c / UPK;
     const int bs = static_cast<int>(a.BS);
     struct Group {
       int page;  // of 16-key group `lane` of a step (lanes 0-7); -1: nothing to see there
@@ -444,16 +480,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       }
       return g;
     };
-    auto load_codes = [&](const uint8_t* cache, const Group& g, int i, uint4 (&x)[NP]) {
+    // this thread's byte offsets of step i in either cache (-1: zeros)
+    auto offsets = [&](const Group& g, int i, int64_t (&off)[NP]) {
+      const int left = T.key_end(i) - T.key(i);
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const int kk = j * RPP + kr;  // key of the step
-        const int page = __shfl_sync(0xffffffffu, g.page, kk >> 4), off = __shfl_sync(0xffffffffu, g.off, kk >> 4);
-        const bool in = page >= 0 && T.key(i) + kk < T.key_end(i);
-        x[j] = in ? __ldg(reinterpret_cast<const uint4*>(cache + page * a.s_page + hk * a.s_head +
-                                                         (off + (kk & 15)) * a.s_pos + u * 16))
-                  : make_uint4(0, 0, 0, 0);
+        const int page = __shfl_sync(0xffffffffu, g.page, kk >> 4), at = __shfl_sync(0xffffffffu, g.off, kk >> 4);
+        off[j] = page >= 0 && kk < left ? page * a.s_page + hk * a.s_head + (at + (kk & 15)) * a.s_pos + u * 16 : -1;
       }
+    };
+    auto load_codes = [&](const uint8_t* cache, const int64_t (&off)[NP], uint4 (&x)[NP]) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+        x[j] = off[j] >= 0 ? __ldg(reinterpret_cast<const uint4*>(cache + off[j])) : make_uint4(0, 0, 0, 0);
     };
     auto store_tile = [&](uint32_t base, const uint4 (&x)[NP]) {
 #pragma unroll
@@ -474,8 +514,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
     };
     Group g0 = load_group(0), g1 = load_group(1);
     uint4 kx[NP], vx[NP];
-    load_codes(a.k, g0, 0, kx);
-    load_codes(a.v, g0, 0, vx);
+    int64_t off[NP];
+    if (T.n_steps > 0) {
+      offsets(g0, 0, off);
+      load_codes(a.k, off, kx);
+      load_codes(a.v, off, vx);
+    }
     for (int i = 0; i < T.n_steps; ++i) {
       const int st = i & 1, ri = i & 7;
       const uint32_t par = static_cast<uint32_t>(((i >> 1) - 1) & 1);
@@ -504,7 +548,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       store_tile(sbase + SM::k(st), kx);
       fence_async_smem();
       pr_arrive(&k_full[st]);
-      if (i + 1 < T.n_steps) load_codes(a.k, g1, i + 1, kx);
+      if (i + 1 < T.n_steps) {
+        offsets(g1, i + 1, off);
+        load_codes(a.k, off, kx);
+      }
       if (KVT != SRSWA_I8) {
         const bool whole = (!T.needs(0, i) || T.whole(0, i)) && (!T.needs(1, i) || T.whole(1, i));
         if (!whole) {
@@ -527,7 +574,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       store_tile(sbase + SM::v(st), vx);
       fence_async_smem();
       pr_arrive(&v_full[st]);
-      if (i + 1 < T.n_steps) load_codes(a.v, g1, i + 1, vx);
+      if (i + 1 < T.n_steps) load_codes(a.v, off, vx);
       g0 = g1;
       g1 = g2;
     }
