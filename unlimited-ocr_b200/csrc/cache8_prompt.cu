@@ -80,7 +80,16 @@ __device__ __noinline__ bool pr_wait_slow(uint32_t bar, uint32_t parity, volatil
 }
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
   const uint32_t a = smem_u32(bar);
-  return mbar_try_wait(a, parity) || pr_wait_slow(a, parity, abort_flag, code);
+  for (int n = 0; n < 4096; ++n) {  // no suspension hint: a step's roles wait for microseconds at most
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return pr_wait_slow(a, parity, abort_flag, code);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -586,14 +595,18 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         if (T.needs(s, i)) last[s] = i;
     bool ok = true;
     int cnt[2] = {0, 0};
+    // descriptors of tile 0 / stage 0; a step in shared memory is a step >> 4 here
+    // (the start address field is 14 bits: everything lies under 256 KB)
+    const uint64_t q_desc = sw128_desc(sbase + SM::q(0), 16, 1024), k_desc = sw128_desc(sbase + SM::k(0), 16, 1024);
+    const uint64_t v_desc = sw128_desc(sbase + SM::v(0), kHalf, 1024);
     auto issue_s = [&](int s, int i) {
       if (!T.needs(s, i)) return;
       constexpr uint32_t id = idesc_f16(128, kPrKeys, 0);
-      const uint32_t qs = sbase + SM::q(s), ks = sbase + SM::k(i & 1);
+      const uint64_t qd = q_desc + (s ? SM::kTile >> 4 : 0), kd = k_desc + (i & 1 ? SM::kTile >> 4 : 0);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
-        const uint32_t off = (x >> 2) * kHalf + (x & 3) * 32u;
-        mma_bf16_ss(tmem + s * 256, sw128_desc(qs + off, 16, 1024), sw128_desc(ks + off, 16, 1024), id, x > 0 ? 1u : 0u);
+        const uint32_t off = ((x >> 2) * kHalf + (x & 3) * 32u) >> 4;
+        mma_bf16_ss(tmem + s * 256, qd + off, kd + off, id, x > 0 ? 1u : 0u);
       }
       mma_commit(&s_full[s]);
       pr_arrive(&s_full[s]);
@@ -603,11 +616,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       if (!pr_wait(&p_full[s], cnt[s] & 1, abort_p, 632)) return false;
       tc_fence_after();
       constexpr uint32_t id = idesc_f16(128, D, 1);
-      const uint32_t vs = sbase + SM::v(i & 1);
+      const uint64_t vd = v_desc + (i & 1 ? SM::kTile >> 4 : 0);
 #pragma unroll
       for (int x = 0; x < kPrKeys / 16; ++x)
-        mma_bf16_ts(tmem + s * 256 + kO, tmem + s * 256 + x * 8, sw128_desc(vs + x * 2048u, kHalf, 1024), id,
-                    cnt[s] > 0 || x > 0 ? 1u : 0u);
+        mma_bf16_ts(tmem + s * 256 + kO, tmem + s * 256 + x * 8, vd + x * 128u, id, cnt[s] > 0 || x > 0 ? 1u : 0u);
       ++cnt[s];
       if (i == last[s]) mma_commit(&o_full[s]);
       return true;
