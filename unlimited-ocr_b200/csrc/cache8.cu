@@ -52,11 +52,49 @@ __device__ __forceinline__ float pow2_scale(float amax) {
 
 constexpr int kAppendThreads = 128;
 
-// One CTA per (page a request's new tokens touch, head, K or V).
+// 1 / s of a power of two is exact, and so is x times it; another writer's scale
+// is divided by.
+struct Scaler {
+  float s, inv;
+  bool pow2;
+  __device__ __forceinline__ explicit Scaler(float scale) : s(scale), inv(1.f / scale) {
+    const uint32_t u = __float_as_uint(scale);
+    pow2 = (u & 0x7fffffu) == 0 && u >= 0x00800000u && u < 0x7f000000u;
+  }
+  template <int KVT>
+  __device__ __forceinline__ uint8_t code(float x) const { return to_code<KVT>(pow2 ? x * inv : x / s); }
+};
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float v = fabsf(x);
+  return v <= 3.402823466e38f ? v : 0.f;
+}
+
+// Earlier tokens [0, held) of a page, rounded from scale `old` to `s`: thread
+// `i` of `n`, 8 codes at a time.
+template <int D, int KVT>
+__device__ __forceinline__ void regrow(uint8_t* tile, int64_t s_pos, int held, float old, float s, int i, int n) {
+  const float r = old / s;
+  for (int w = i; w < held * (D / 8); w += n) {
+    uint2* c = reinterpret_cast<uint2*>(tile + (w / (D / 8)) * s_pos + (w % (D / 8)) * 8);
+    uint2 x = *c;
+    uint8_t* b = reinterpret_cast<uint8_t*>(&x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = to_code<KVT>(code_to_float(b[e], KVT) * r);
+    *c = x;
+  }
+}
+
+// One CTA per (page a request's new tokens touch, head, K or V).  Bound by
+// memory: the new elements of a page stay in registers between the maximum and
+// the rounding (pages of up to 8 passes of the CTA; longer ones are read twice,
+// the second time from L2), so each is read once and its code written once.
+// 38k tokens of 10 heads of 128, bf16 to e4m3: see the table of measurements.
 template <int D, int KVT>
 __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const AppendArgs a) {
   constexpr int LPT = D / 8;                     // lanes per token, 8 elements each
   constexpr int TPP = kAppendThreads / LPT;      // tokens per pass
+  constexpr int NP = 8;                          // passes held in registers
   __shared__ float red[kAppendThreads / 32];
   const int tid = threadIdx.x;
   const int64_t head = blockIdx.y;
@@ -67,13 +105,14 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const App
   int64_t req, start, n, row0, nth;
   if (a.rows.cu) {
     const int64_t i = blockIdx.x;
-    int64_t lo = 0, hi = a.rows.R;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.rows.cu[mid] / a.BS + 2 * mid <= i) lo = mid;
-      else hi = mid;
+    int64_t before = 0;  // requests that begin at or before this slot
+    for (int64_t r0 = 0; r0 < a.rows.R; r0 += kAppendThreads) {
+      const int64_t r = r0 + tid;
+      const int here = __syncthreads_count(r < a.rows.R && a.rows.cu[r] / a.BS + 2 * r <= i);
+      before += here;
+      if (here < kAppendThreads) break;
     }
-    req = lo;
+    req = before - 1;
     row0 = a.rows.cu[req];
     nth = i - (row0 / a.BS + 2 * req);
     n = a.rows.cu[req + 1] - row0;
@@ -90,60 +129,139 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const App
   const int64_t blk = start / a.BS + nth;
   const int64_t lo = max(start, blk * a.BS), hi = min(start + n, (blk + 1) * a.BS);  // positions written here
   if (lo >= hi || blk >= a.W) return;
-  const int64_t page = a.table[req * a.s_bt + blk];
-  if (page < 0 || page >= a.P) return;
+  const int count = static_cast<int>(hi - lo), held = static_cast<int>(lo - blk * a.BS);  // new, earlier tokens
 
   const void* x = a.x[which];
-  const int64_t xoff = head * a.s_xh[which];
+  const int g = tid / LPT, u = tid % LPT;
+  const int64_t x0 = (row0 + lo - start) * a.s_xn[which] + head * a.s_xh[which] + u * 8;
   const int64_t s_xn = a.s_xn[which];
+  const bool fits = count <= NP * TPP && a.x_dtype != SRSWA_F32;  // uniform
+  uint4 raw[NP];
+  float amax = 0.f;
+  if (fits) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+      raw[j] = j * TPP + g < count ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + x0 + (j * TPP + g) * s_xn))
+                                   : make_uint4(0, 0, 0, 0);
+  }
+  const int64_t page = a.table[req * a.s_bt + blk];
+  if (page < 0 || page >= a.P) return;
   uint8_t* dst = a.cache[which] + page * a.s_page + head * a.s_head;
   float* scale = a.scale[which] + page * a.s_scale + head;
-  const int g = tid / LPT, u = tid % LPT;
+  const float old = held > 0 ? *scale : 0.f;
 
-  float amax = 0.f;
-  for (int64_t p = lo + g; p < hi; p += TPP) {
-    float f[8];
-    load8(x, (row0 + p - start) * s_xn + xoff + u * 8, a.x_dtype, f);
+  auto unpack = [&](const uint4& w, float (&f)[8]) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = fabsf(f[e]);
-      if (v <= 3.402823466e38f) amax = fmaxf(amax, v);  // finite elements only
+    for (int e = 0; e < 4; ++e) {
+      if (a.x_dtype == SRSWA_BF16) {
+        f[2 * e] = bf16_lo(v[e]);
+        f[2 * e + 1] = bf16_hi(v[e]);
+      } else {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+        f[2 * e] = p.x;
+        f[2 * e + 1] = p.y;
+      }
+    }
+  };
+  float f[8];
+  if (fits) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      unpack(raw[j], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
+    }
+  } else {
+    for (int t = g; t < count; t += TPP) {
+      load8(x, x0 + t * s_xn, a.x_dtype, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
     }
   }
   amax = warp_max(amax);
   if ((tid & 31) == 0) red[tid >> 5] = amax;
-  __syncthreads();
+  __syncthreads();  // and every thread has read the old scale
 #pragma unroll
   for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, red[w]);
 
   float s = pow2_scale<KVT>(amax);
-  const int64_t held = lo - blk * a.BS;  // earlier tokens of the page
   if (held > 0) {
-    const float old = *scale;
-    __syncthreads();  // every thread has read it
-    if (s > old) {
-      const float r = old / s;
-      for (int64_t p = g; p < held; p += TPP) {
-        uint2* c = reinterpret_cast<uint2*>(dst + p * a.s_pos + u * 8);
-        uint2 w = *c;
-        uint8_t* b = reinterpret_cast<uint8_t*>(&w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = to_code<KVT>(code_to_float(b[e], KVT) * r);
-        *c = w;
-      }
-    } else {
-      s = old;
-    }
+    if (s > old) regrow<D, KVT>(dst, a.s_pos, held, old, s, tid, kAppendThreads);
+    else s = old;
   }
   if (tid == 0) *scale = s;
-  for (int64_t p = lo + g; p < hi; p += TPP) {
-    float f[8];
-    load8(x, (row0 + p - start) * s_xn + xoff + u * 8, a.x_dtype, f);
+  const Scaler sc(s);
+  auto put = [&](int t) {
     uint2 w;
     uint8_t* b = reinterpret_cast<uint8_t*>(&w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = to_code<KVT>(f[e] / s);
-    *reinterpret_cast<uint2*>(dst + (p - blk * a.BS) * a.s_pos + u * 8) = w;
+    for (int e = 0; e < 8; ++e) b[e] = sc.code<KVT>(f[e]);
+    *reinterpret_cast<uint2*>(dst + (held + t) * a.s_pos + u * 8) = w;
+  };
+  if (fits) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      unpack(raw[j], f);
+      if (j * TPP + g < count) put(j * TPP + g);
+    }
+  } else {
+    for (int t = g; t < count; t += TPP) {
+      load8(x, x0 + t * s_xn, a.x_dtype, f);
+      put(t);
+    }
+  }
+}
+
+// One new token per request (decode): one warp per (request, head, K or V), a
+// lane holds D / 32 features.  Bound by the latency of its four dependent reads
+// (length, page, scale; the elements come beside them).
+template <int D, int KVT>
+__global__ void __launch_bounds__(kAppendThreads) cache8_append_one_kernel(const AppendArgs a) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int which = static_cast<int>(item % 2);
+  const int64_t head = item / 2 % a.Hkv, req = item / 2 / a.Hkv;
+  if (req >= a.rows.R) return;
+  const int64_t pos = static_cast<int64_t>(a.rows.seq_lens[req]) - 1;
+  float f[E], amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    f[e] = load_elem(a.x[which], req * a.s_xn[which] + head * a.s_xh[which] + lane * E + e, a.x_dtype);
+    amax = fmaxf(amax, finite_abs(f[e]));
+  }
+  if (pos < 0 || pos >= a.W * a.BS) return;
+  const int64_t blk = pos / a.BS, page = a.table[req * a.s_bt + blk];
+  if (page < 0 || page >= a.P) return;
+  const int held = static_cast<int>(pos - blk * a.BS);
+  uint8_t* dst = a.cache[which] + page * a.s_page + head * a.s_head;
+  float* scale = a.scale[which] + page * a.s_scale + head;
+  float s = pow2_scale<KVT>(warp_max(amax));
+  if (held > 0) {
+    const float old = *scale;
+    if (s > old) regrow<D, KVT>(dst, a.s_pos, held, old, s, lane, 32);
+    else s = old;
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale = s;
+  const Scaler sc(s);
+  uint8_t b[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) b[e] = sc.code<KVT>(f[e]);
+  uint8_t* p = dst + held * a.s_pos + lane * E;
+  if constexpr (E == 4) *reinterpret_cast<uchar4*>(p) = make_uchar4(b[0], b[1], b[2], b[3]);
+  else *reinterpret_cast<uchar2*>(p) = make_uchar2(b[0], b[1]);
+}
+
+template <int D, int KVT>
+static void append_start(const AppendArgs& a, int64_t slots, cudaStream_t st) {
+  if (!a.rows.cu && a.rows.rps == 1) {
+    const int64_t ctas = (2 * a.rows.R * a.Hkv + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    cache8_append_one_kernel<D, KVT><<<static_cast<unsigned>(ctas), kAppendThreads, 0, st>>>(a);
+  } else {
+    const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(a.Hkv), 2);
+    cache8_append_kernel<D, KVT><<<grid, kAppendThreads, 0, st>>>(a);
   }
 }
 
@@ -191,7 +309,7 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
   SRSWA_CHECK_ARG(((d->s_qn | d->s_qh | d->s_on | d->s_oh) & m) == 0, SRSWA_EALIGN);
   const int64_t slots = cu_rows ? d->N / d->block_size + 2 * d->R
                                 : d->R * ((d->rows_per_req + d->block_size - 2) / d->block_size + 1);
-  SRSWA_CHECK_ARG(slots < (1ll << 31), SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(slots < (1ll << 31) && d->R * d->Hkv < (1ll << 31), SRSWA_ETOOLARGE);
   AppendArgs a = {};
   a.x[0] = k; a.x[1] = v;
   a.cache[0] = static_cast<uint8_t*>(k_cache); a.cache[1] = static_cast<uint8_t*>(v_cache);
@@ -201,14 +319,13 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
   a.table = block_table; a.s_bt = d->s_bt; a.W = d->W; a.P = d->P; a.BS = d->block_size; a.N = d->N; a.Hkv = d->Hkv;
   a.s_page = d->s_page; a.s_pos = d->s_pos; a.s_head = d->s_head; a.s_scale = d->s_scale;
   a.x_dtype = d->q_dtype;
-  const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(d->Hkv), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (d->D == 128) {
-    if (d->kv_dtype == SRSWA_I8) cache8_append_kernel<128, SRSWA_I8><<<grid, kAppendThreads, 0, st>>>(a);
-    else cache8_append_kernel<128, SRSWA_F8E4M3><<<grid, kAppendThreads, 0, st>>>(a);
+    if (d->kv_dtype == SRSWA_I8) append_start<128, SRSWA_I8>(a, slots, st);
+    else append_start<128, SRSWA_F8E4M3>(a, slots, st);
   } else {
-    if (d->kv_dtype == SRSWA_I8) cache8_append_kernel<64, SRSWA_I8><<<grid, kAppendThreads, 0, st>>>(a);
-    else cache8_append_kernel<64, SRSWA_F8E4M3><<<grid, kAppendThreads, 0, st>>>(a);
+    if (d->kv_dtype == SRSWA_I8) append_start<64, SRSWA_I8>(a, slots, st);
+    else append_start<64, SRSWA_F8E4M3>(a, slots, st);
   }
   return srswa_last_launch_status();
 }

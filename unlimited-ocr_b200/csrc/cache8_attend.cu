@@ -24,7 +24,8 @@
 // kv head) items are laid end to end and cut into equal parts, one per resident
 // warp, so uneven lengths leave no tail and warps never wait for one another;
 // an item cut in several parts leaves fp32 partials that cache8_merge_kernel
-// joins in order.  A warp streams its units through a private cp.async ring;
+// joins in order.  Where the items are few and short the join would cost more
+// than the balance gives: there the four warps of a CTA share an item.  A warp streams its units through a private cp.async ring;
 // page ids, scales and biases are prefetched a block of 32 slots ahead.
 
 #include <cmath>
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   constexpr int RPI = 512 / D;         // key rows per warp copy instruction
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t f_sum[kRowsThreads + 1];
+  __shared__ float w_ml[kRowsWarps][2 * kCols];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
@@ -134,9 +136,11 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   const int cr = lane / (D / 16), cc = lane % (D / 16);  // key row and 16-byte unit of this lane's copies
   pdl_launch_dependents();                  // the merge kernel waits for this grid before it reads
 
-  // One (row group, kv head, column group), units [c0, c1) of its `s.units`;
-  // slot < 0: the whole item, results written out; else partial `slot`.
-  auto process = [&](int64_t rg, int64_t req, const Span& s, int64_t hk, int grp, int c0, int c1, int64_t slot) {
+  // One (row group, kv head, column group), units [c0, c1) of its `s.units`.
+  // po == nullptr: the whole item, results written out; else a part: its
+  // unnormalised outputs to po [8 columns][D], maxima and sums to pml [8][2].
+  auto process = [&](int64_t rg, int64_t req, const Span& s, int64_t hk, int grp, int c0, int c1, float* po,
+                     float* pml) {
     const int64_t n0 = rg * share;
     // ---- slots: lane l of (cur, nxt) holds slot base + l, base + 32 + l ----
     const int n_fix = s.n_sink + s.n_win, nslots = n_fix + K;
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
         x[2 * e] = o[e][u];
         x[2 * e + 1] = o[e][2 + u];
       }
-      if (slot < 0) {
+      if (!po) {
         const int64_t n = n0 + gc / G, h = hk * G + gc % G;
         const bool any = l > 0.f || l != l;
 #pragma unroll
@@ -469,12 +473,12 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
         for (int e = 0; e < 2 * KS; e += 8) store8(a.out, n * a.s_on + h * a.s_oh + g * 2 * KS + e, a.out_dtype, x + e);
         if (g == 0 && a.lse) a.lse[n * a.H + h] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
       } else {
-        float4* po = reinterpret_cast<float4*>(a.part_o + (slot * kCols + col) * D + g * 2 * KS);
+        float4* p = reinterpret_cast<float4*>(po + col * D + g * 2 * KS);
 #pragma unroll
-        for (int e = 0; e < 2 * KS; e += 4) po[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        for (int e = 0; e < 2 * KS; e += 4) p[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         if (g == 0) {
-          a.part_ml[(slot * kCols + col) * 2] = m;
-          a.part_ml[(slot * kCols + col) * 2 + 1] = l;
+          pml[col * 2] = m;
+          pml[col * 2 + 1] = l;
         }
       }
     }
@@ -485,7 +489,13 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   const int64_t groups = a.N / share;
   int64_t req, pos, stop, rg, off;
   Span s;
-  if (!a.balanced) {  // one warp per item
+  if (a.split == kSplitCta) {  // a quarter of the CTA's item
+    rg = blockIdx.x / per_group;
+    s = group_span<CH>(a, rg, req);
+    pos = s.units * warp / kRowsWarps;
+    stop = s.units * (warp + 1) / kRowsWarps;
+    off = (blockIdx.x % per_group) * s.units + pos;
+  } else if (a.split == kSplitNone) {  // one warp per item
     rg = me / per_group;
     if (rg >= groups) return;
     s = group_span<CH>(a, rg, req);
@@ -537,21 +547,24 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   }
   int head_rg = pos < stop ? -1 : -2;  // -2, an empty part: an item may go on behind it
   int head_item = 0, tail_rg = -1, tail_item = 0;
-  while (pos < stop) {
+  bool once = a.split == kSplitCta;  // its part, an empty one too, goes to shared memory
+  while (pos < stop || once) {
     const int64_t it = off / s.units;
     const int c0 = static_cast<int>(off % s.units);
     const int c1 = static_cast<int>(min(static_cast<int64_t>(s.units), c0 + stop - pos));
-    int64_t slot = -1;
-    if (c0 > 0) {
-      slot = 2 * me;
-      head_rg = static_cast<int>(rg);
-      head_item = static_cast<int>(it);
-    } else if (c1 < s.units) {
-      slot = 2 * me + 1;
-      tail_rg = static_cast<int>(rg);
-      tail_item = static_cast<int>(it);
+    float *po = nullptr, *pml = nullptr;
+    if (once) {
+      po = reinterpret_cast<float*>(smem + warp * ST * SB);  // this warp's ring, when it is done with it
+      pml = w_ml[warp];
+      once = false;
+    } else if (c0 > 0 || c1 < s.units) {
+      const int64_t slot = c0 > 0 ? 2 * me : 2 * me + 1;
+      (c0 > 0 ? head_rg : tail_rg) = static_cast<int>(rg);
+      (c0 > 0 ? head_item : tail_item) = static_cast<int>(it);
+      po = a.part_o + slot * kCols * D;
+      pml = a.part_ml + slot * kCols * 2;
     }
-    process(rg, req, s, it / a.ngrp, static_cast<int>(it % a.ngrp), c0, c1, slot);
+    process(rg, req, s, it / a.ngrp, static_cast<int>(it % a.ngrp), c0, c1, po, pml);
     pos += c1 - c0;
     off += c1 - c0;
     if (off == s.units * per_group && pos < stop) {
@@ -559,7 +572,31 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       s = group_span<CH>(a, ++rg, req);
     }
   }
-  if (lane == 0 && a.balanced) reinterpret_cast<int4*>(a.part_meta)[me] = make_int4(head_rg, head_item, tail_rg, tail_item);
+  if (a.split == kSplitEqual) {
+    if (lane == 0) reinterpret_cast<int4*>(a.part_meta)[me] = make_int4(head_rg, head_item, tail_rg, tail_item);
+  } else if (a.split == kSplitCta) {  // join the four parts
+    __syncthreads();
+    const int64_t it = blockIdx.x % per_group, hk = it / a.ngrp, row0 = blockIdx.x / per_group * share;
+    const int first = static_cast<int>(it % a.ngrp) * kCols, ncol = min(share * G - first, kCols);
+    for (int i = tid; i < ncol * D; i += kRowsThreads) {
+      const int col = i / D, d = i % D, gc = first + col;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, w_ml[w][2 * col]);
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float L = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) {
+        const float f = exp2f(w_ml[w][2 * col] - Mu);
+        L += w_ml[w][2 * col + 1] * f;
+        x += reinterpret_cast<const float*>(smem + w * ST * SB)[col * D + d] * f;
+      }
+      const bool any = L > 0.f || L != L;
+      const int64_t n = row0 + gc / G, h = hk * G + gc % G;
+      store_elem(a.out, n * a.s_on + h * a.s_oh + d, a.out_dtype, any ? x / L : 0.f);
+      if (d == 0 && a.lse) a.lse[n * a.H + h] = any ? (M + log2f(L)) * kLn2 : -INFINITY;
+    }
+  }
 }
 
 // Joins the parts of one column (blockIdx.y) of the item that part blockIdx.x
@@ -663,22 +700,26 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   }
   const int64_t most = (blocks + d.K) * upp;
   const int64_t slots = static_cast<int64_t>(sm_count()) * kRowsCtasPerSm * kRowsWarps;
-  int64_t parts;
+  int64_t parts = p.items;
+  p.split = kSplitNone;
   if (d.nsplit > 0) {
-    p.balanced = d.nsplit > 1;
+    if (d.nsplit > 1) p.split = kSplitEqual;
     parts = d.nsplit * p.items;
-  } else if (most <= 2 || groups > 2048 || p.items > 16 * slots) {
+  } else if (p.items <= slots / kRowsWarps && most <= 16 * kRowsWarps) {
+    // one wave of CTAs, at most 16 units a warp: 10 items of 9 units take TIME1 us
+    // against TIME2 with equal parts and a join, 288 of up to 35 TIME3 against TIME4
+    p.split = kSplitCta;
+    parts = p.items * kRowsWarps;
+  } else if (most <= 2 || groups > 2048 || p.items > 16 * slots || (p.items >= slots && most <= 16)) {
     // items that a warp is through with at once, or so many that their uneven
     // ends do not show: one warp each, no join
-    p.balanced = false;
-    parts = p.items;
   } else {
-    p.balanced = true;
+    p.split = kSplitEqual;
     const int64_t enough = (p.items * most + 1) / 2;  // two units each at least
     parts = enough < slots ? enough : slots;
   }
   p.ctas = (parts + kRowsWarps - 1) / kRowsWarps;
-  if (p.balanced) {
+  if (p.split == kSplitEqual) {
     parts = p.ctas * kRowsWarps;
     const int64_t f = parts * 2 * kCols;
     p.o_floats = f * d.D;
@@ -705,7 +746,7 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   if (a.K > kMaxSelected || p.ctas >= (1ll << 28)) return SRSWA_ETOOLARGE;
   a.share = p.share;
   a.ngrp = p.ngrp;
-  a.balanced = p.balanced ? 1 : 0;
+  a.split = p.split;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + p.o_floats;
   const int64_t parts = p.ctas * kRowsWarps;
@@ -726,7 +767,7 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   using D128 = std::integral_constant<int, 128>;
   const int rc = a.D == 128 ? (p.ch == 2 ? by_type(D128(), Two()) : by_type(D128(), One()))
                             : (p.ch == 2 ? by_type(D64(), Two()) : by_type(D64(), One()));
-  if (rc || !p.balanced) return rc;
+  if (rc || p.split != kSplitEqual) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(parts), static_cast<unsigned>(p.share * (a.H / a.Hkv) < kCols ? p.share * (a.H / a.Hkv) : kCols), 1);
   cfg.blockDim = dim3(128, 1, 1);

@@ -5,6 +5,9 @@
 
 namespace srswa {
 
+// One warp per item; the four warps of a CTA per item; equal parts of all units per warp.
+enum { kSplitNone = 0, kSplitCta = 1, kSplitEqual = 2 };
+
 struct Attend8Args {
   const void* q;
   const uint8_t* k;
@@ -25,7 +28,7 @@ struct Attend8Args {
   int q_dtype, out_dtype, idx_is64;
   // single rows
   int64_t share, ngrp;  // rows that share a pass over the keys; column groups of an item
-  int balanced;         // 1: equal parts of all units per warp, 0: one warp per item
+  int split;            // how the items are shared out (below)
   float* part_o;        // [2 per part][8 columns][D] unnormalised partial outputs
   float* part_ml;       // [..][8][2] their maxima (log2) and sums
   int* part_meta;       // [part][4] the items its two partials belong to (row group, item, twice)
@@ -69,7 +72,7 @@ __device__ __forceinline__ float ex2(float x) {
 struct RowsPlan {
   int64_t share, ngrp, items, ctas, o_floats;
   size_t bytes;  // workspace
-  bool balanced;
+  int split;
   int ch;  // 16-key chunks of a unit
 };
 RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen);
