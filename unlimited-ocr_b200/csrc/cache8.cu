@@ -29,6 +29,17 @@ struct AppendArgs {
   int x_dtype;
 };
 
+// Two elements -> two codes (the first in the low byte).
+template <int KVT>
+__device__ __forceinline__ uint32_t to_code2(float x, float y) {
+  if (KVT == SRSWA_I8) {
+    const int a = x != x ? 0 : __float2int_rn(fminf(fmaxf(x, -127.f), 127.f));
+    const int b = y != y ? 0 : __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
+    return (static_cast<uint32_t>(a) & 0xffu) | ((static_cast<uint32_t>(b) & 0xffu) << 8);
+  }
+  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+}
+
 template <int KVT>
 __device__ __forceinline__ uint8_t to_code(float y) {
   if (KVT == SRSWA_I8) {
@@ -150,27 +161,41 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const App
   float* scale = a.scale[which] + page * a.s_scale + head;
   const float old = held > 0 ? *scale : 0.f;
 
-  auto unpack = [&](const uint4& w, float (&f)[8]) {
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (a.x_dtype == SRSWA_BF16) {
-        f[2 * e] = bf16_lo(v[e]);
-        f[2 * e + 1] = bf16_hi(v[e]);
-      } else {
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
-        f[2 * e] = p.x;
-        f[2 * e + 1] = p.y;
-      }
-    }
+  auto unpack = [&](uint32_t w) {
+    if (a.x_dtype == SRSWA_BF16) return make_float2(bf16_lo(w), bf16_hi(w));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
   };
   float f[8];
   if (fits) {
+    // the largest magnitude in the elements' own type, two at a time (its maximum
+    // skips NaN); an infinity among them is rare and sends us over them again
+    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      unpack(raw[j], f);
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t v = w[e] & 0x7fff7fffu;
+        if (a.x_dtype == SRSWA_BF16) {
+          const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&top),
+                                           *reinterpret_cast<const __nv_bfloat162*>(&v));
+          top = *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+          const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&top), *reinterpret_cast<const __half2*>(&v));
+          top = *reinterpret_cast<const uint32_t*>(&r);
+        }
+      }
+    }
+    const float2 t2 = unpack(top);
+    amax = fmaxf(t2.x, t2.y);
+    if (!(amax <= 3.402823466e38f)) {
+      amax = 0.f;
+#pragma unroll 1
+      for (int t = g; t < count; t += TPP) {
+        load8(x, x0 + t * s_xn, a.x_dtype, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
+      }
     }
   } else {
     for (int t = g; t < count; t += TPP) {
@@ -192,23 +217,29 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const App
   }
   if (tid == 0) *scale = s;
   const Scaler sc(s);
-  auto put = [&](int t) {
-    uint2 w;
-    uint8_t* b = reinterpret_cast<uint8_t*>(&w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = sc.code<KVT>(f[e]);
-    *reinterpret_cast<uint2*>(dst + (held + t) * a.s_pos + u * 8) = w;
-  };
-  if (fits) {
+  uint8_t* out = dst + held * a.s_pos + u * 8;
+  if (fits && sc.pow2) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      unpack(raw[j], f);
-      if (j * TPP + g < count) put(j * TPP + g);
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      uint32_t c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = unpack(w[e]);
+        c[e] = to_code2<KVT>(v.x * sc.inv, v.y * sc.inv);
+      }
+      if (j * TPP + g < count)
+        *reinterpret_cast<uint2*>(out + (j * TPP + g) * a.s_pos) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
     }
   } else {
+#pragma unroll 1
     for (int t = g; t < count; t += TPP) {
       load8(x, x0 + t * s_xn, a.x_dtype, f);
-      put(t);
+      uint2 w;
+      uint8_t* b = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = sc.code<KVT>(f[e]);
+      *reinterpret_cast<uint2*>(out + t * a.s_pos) = w;
     }
   }
 }
