@@ -959,13 +959,13 @@ def cache8_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=N
         qs = q.stride()
     out_type = real
     if out is None:
-        out = torch.empty(shape, device=dev, dtype=q.dtype)
-        os_ = (H * D, D)
+        out = torch.empty_like(q)  # q's order of rows and heads, if it has no gaps
+        os_ = out.stride()
     else:
         if out.shape != shape or out.device != dev or out.stride(2) != 1 or out.dtype not in (q.dtype, torch.float32):
             raise ValueError(f"out must be {tuple(shape)} of q's type or fp32, features contiguous, on {dev}")
         os_, out_type = out.stride(), _REALS[out.dtype]
-    lse_t = torch.empty((N, H), device=dev, dtype=torch.float32) if lse else None
+    lse_t = torch.empty_strided((N, H), (H, 1), device=dev, dtype=torch.float32) if lse else None
     if window is None:
         window = -1
     elif window < 0:
@@ -1004,7 +1004,7 @@ def cache8_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=N
     need = lib.srswa_cache8_attend_workspace_size(d, 0 if cu is None else 1)
     ws = None
     if need:
-        ws = (torch.empty(need, device=dev, dtype=torch.uint8) if workspace is None
+        ws = (torch.empty_strided((need,), (1,), device=dev, dtype=torch.uint8) if workspace is None
               else _workspace(need, dev, workspace)).data_ptr()
     rc = lib.srswa_cache8_attend(d, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                                  v_scale.data_ptr(), block_table.data_ptr(), sl, cu, pl, ti, bi, out.data_ptr(),
@@ -1034,15 +1034,14 @@ def _page_tensors(tensors, P, dev):
     run of bytes (the other dimensions in any order, none padded)."""
     words = []
     for i, t in enumerate(tensors):
-        shape = t.shape
+        shape, st = t.shape, t.stride()
         if len(shape) == 0 or shape[0] != P or t.get_device() != dev:
             raise ValueError(f"tensor {i}: {tuple(shape)} is not indexed by {P} pages on the table's device")
-        es = t.element_size()
-        st = t.stride()
         if t.is_contiguous() or (len(shape) == 4 and st[3] == 1 and st[1] == shape[3] and st[2] == shape[1] * shape[3]
                                  and st[0] == shape[2] * st[2]):  # (page, head) tiles
-            n = step = t.numel() // P if P else 0
+            n = step = t.nbytes // P if P else 0
         else:
+            es = t.element_size()
             n = 1
             for size, stride in sorted(zip(shape[1:], st[1:]), key=lambda x: x[1]):
                 if size != 1 and stride != n:
@@ -1051,9 +1050,16 @@ def _page_tensors(tensors, P, dev):
                 n *= size
             if P > 1 and st[0] < n:
                 raise ValueError(f"tensor {i}: pages overlap: {tuple(shape)} with strides {st}")
-            step = max(st[0], n)
-        words += (t.data_ptr(), n * es, step * es)
+            n, step = n * es, max(st[0], n) * es
+        words += (t.data_ptr(), n, step)
     return struct.pack(f"@{len(words)}q", *words) if words else None
+
+
+def _page_scratch(n, dev):
+    """A one-element result and n ints of scratch (empty_strided: the cheapest
+    way to them, a microsecond less each than empty)."""
+    return (torch.empty_strided((1,), (1,), device=dev, dtype=torch.int32),
+            torch.empty_strided((n,), (1,), device=dev, dtype=torch.int32))
 
 
 def pages_free(rows, block_table, seq_lens, refs, *, block_size):
@@ -1077,8 +1083,7 @@ def pages_extend(rows, new_lens, block_table, seq_lens, refs, *, block_size):
     if new_lens.shape[0] != n:
         raise ValueError("rows and new_lens must be equally long")
     stream = L.stream_of(block_table)
-    short = torch.empty(1, device=rows.device, dtype=torch.int32)
-    ws = torch.empty(n + R + P, device=rows.device, dtype=torch.int32)
+    short, ws = _page_scratch(n + R + P, rows.device)
     rc = L.lib().srswa_pages_extend(rows.data_ptr(), new_lens.data_ptr(), n, bt, s_bt, R, W, seq_lens.data_ptr(),
                                     refs.data_ptr(), P, block_size, short.data_ptr(), ws.data_ptr(), 4 * (n + R + P),
                                     stream)
@@ -1099,8 +1104,7 @@ def pages_fork(parents, children, block_table, seq_lens, refs, tensors, *, block
         raise ValueError("parents and children must be equally long")
     arr = _page_tensors(tensors, P, block_table.get_device())
     stream = L.stream_of(block_table)
-    short = torch.empty(1, device=parents.device, dtype=torch.int32)
-    ws = torch.empty(n + R + P, device=parents.device, dtype=torch.int32)
+    short, ws = _page_scratch(n + R + P, parents.device)
     rc = L.lib().srswa_pages_fork(parents.data_ptr(), children.data_ptr(), n, bt, s_bt, R, W, seq_lens.data_ptr(),
                                   refs.data_ptr(), P, block_size, arr, len(tensors), short.data_ptr(), ws.data_ptr(),
                                   4 * (n + R + P), stream)
@@ -1118,20 +1122,19 @@ def pages_compact(block_table, refs, tensors, *, out_table=None, out_refs=None):
     bt, s_bt, R, W, P = _page_args(block_table, None, refs)
     dev = block_table.device
     if out_table is None:
-        out_table = torch.empty((R, W), device=dev, dtype=torch.int32)
+        out_table = torch.empty_strided((R, W), (W, 1), device=dev, dtype=torch.int32)
     elif (out_table.shape != (R, W) or out_table.dtype != torch.int32 or out_table.device != dev
           or (out_table.stride(1) != 1 and W > 1)):
         raise ValueError(f"out_table must be {(R, W)} int32 with contiguous rows on {dev}")
     if out_refs is None:
-        out_refs = torch.empty(P, device=dev, dtype=torch.int32)
+        out_refs = torch.empty_like(refs)
     elif out_refs.shape != (P,) or out_refs.dtype != torch.int32 or not out_refs.is_contiguous() or out_refs.device != dev:
         raise ValueError(f"out_refs must be contiguous int32 [{P}] on {dev}")
     arr = _page_tensors(tensors, P, block_table.get_device())
     stream = L.stream_of(block_table)
-    live = torch.empty(1, device=dev, dtype=torch.int32)
     lib = L.lib()
     need = lib.srswa_pages_compact_workspace_size(P)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    live, ws = _page_scratch(need // 4, dev)
     rc = lib.srswa_pages_compact(bt, s_bt, R, W, refs.data_ptr(), P, arr, len(tensors), out_table.data_ptr(),
                                  out_table.stride(0), out_refs.data_ptr(), live.data_ptr(), ws.data_ptr(), need, stream)
     if rc:
