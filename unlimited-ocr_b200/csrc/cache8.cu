@@ -102,7 +102,7 @@ __device__ __forceinline__ void regrow(uint8_t* tile, int64_t s_pos, int held, f
 // the second time from L2), so each is read once and its code written once.
 // 38k tokens of 10 heads of 128, bf16 to e4m3: see the table of measurements.
 template <int D, int KVT>
-__global__ void __launch_bounds__(kAppendThreads) cache8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const AppendArgs a) {
   constexpr int LPT = D / 8;                     // lanes per token, 8 elements each
   constexpr int TPP = kAppendThreads / LPT;      // tokens per pass
   constexpr int NP = 8;                          // passes held in registers
