@@ -150,20 +150,11 @@ def test_page_tensor_layouts():
     """Pages may be permuted inside, and lie apart; bytes and strides follow."""
     t = torch.zeros(6, 2, 64, 16, dtype=torch.bfloat16).transpose(1, 2)
     x = torch.zeros(6, 2, 3, 4, 5).permute(0, 3, 1, 4, 2)
-    arr = (L.PageTensor * 4).from_buffer_copy(ops._page_tensors([t, torch.zeros(6, 10)[:, :3], torch.zeros(6), x], 6, -1))
-    assert (arr[0].base, arr[0].page_bytes, arr[0].stride_bytes) == (t.data_ptr(), 4096, 4096)
-    assert (arr[1].page_bytes, arr[1].stride_bytes) == (12, 40)
-    assert (arr[2].page_bytes, arr[2].stride_bytes) == (4, 4)
-    assert (arr[3].page_bytes, arr[3].stride_bytes) == (480, 480)
-
-
-def test_descriptor_packing():
-    """The packed descriptor is the ctypes structure, field by field."""
-    names = [n for n, _ in L.Cache8Desc._fields_]
-    raw = ops._DESC8(*[float(i) if n == "sm_scale" else i + 1 for i, n in enumerate(names)])
-    assert len(raw) == C.sizeof(L.Cache8Desc)
-    d = L.Cache8Desc.from_buffer_copy(raw)
-    assert [getattr(d, n) for n in names] == [float(i) if n == "sm_scale" else i + 1 for i, n in enumerate(names)]
+    runs = L.bind().page_runs([t, torch.zeros(6, 10)[:, :3], torch.zeros(6), x, torch.zeros(6, 1, 7)], 6)
+    assert runs[0] == (t.data_ptr(), 4096, 4096) and runs[1][1:] == (12, 40) and runs[2][1:] == (4, 4)
+    assert runs[3][1:] == (480, 480) and runs[4][1:] == (28, 28)
+    with pytest.raises(ValueError):
+        L.bind().page_runs([torch.zeros(6, 4, 8)[:, :, ::2]], 6)
 
 
 def test_oracle_codes_match_torch():

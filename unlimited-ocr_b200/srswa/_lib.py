@@ -190,6 +190,24 @@ def lib():
     return _lib
 
 
+_bound = None
+
+
+def bind():
+    """The native binding of the cache8 / pages calls (_bind.so, built beside
+    libsrswa.so), pointed at the library that lib() has loaded; raises if it is
+    absent."""
+    global _bound
+    if _bound is None:
+        try:
+            from . import _bind
+        except ImportError as e:
+            raise SrswaError(f"srswa._bind not found ({e}); build it with `python unlimited-ocr_b200/csrc/build.py`") from None
+        _bind.init(lib()._handle, SrswaError)
+        _bound = _bind
+    return _bound
+
+
 def exported_symbols():
     return list(_SIGS)
 

@@ -9,7 +9,6 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
-import struct
 
 import torch
 
@@ -841,94 +840,19 @@ def rope2d_decode_(new_ids, page_id, page, tok, pf_cnt, n_pg):
 
 
 # ------------------------------------------------------- scaled 8-bit cache
-_CODES = {torch.float8_e4m3fn: L.F8E4M3, torch.int8: L.I8}
-_REALS = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
-_DESC8 = struct.Struct("@12qf4i14q").pack  # srswa_cache8_desc (L.Cache8Desc), field by field in one call
-
-
-def _cache8_args(x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens):
-    """What append and attend share: the checks, and (R, Hkv, D, P, W, BS,
-    rows per request, x's type, code type, cache strides, scale and table row
-    strides, the row tensors' pointers).  Plain ints throughout: a decode step
-    makes these calls once per layer."""
-    dev = x.get_device()
-    ds, st, kt = k_cache.shape, k_cache.stride(), k_cache.dtype
-    if len(ds) != 4 or v_cache.shape != ds or v_cache.dtype != kt:
-        raise ValueError("k_cache and v_cache must be [pages, block_size, kv heads, head dim] of one type")
-    P, BS, Hkv, D = ds
-    code, real = _CODES.get(kt), _REALS.get(x.dtype)
-    if code is None:
-        raise NotImplementedError(f"codes of {kt} not supported (float8_e4m3fn or int8)")
-    if real is None:
-        raise NotImplementedError(f"dtype {x.dtype} not supported")
-    if v_cache.stride() != st or st[3] != 1:
-        raise ValueError("k_cache and v_cache must share their strides, features contiguous")
-    ss, ps = k_scale.stride(), (P, Hkv)
-    if (k_scale.shape != ps or v_scale.shape != ps or k_scale.dtype != torch.float32
-            or v_scale.dtype != torch.float32 or v_scale.stride() != ss or (ss[1] != 1 and Hkv > 1)):
-        raise ValueError("k_scale and v_scale must be [pages, kv heads] fp32 with one row stride, heads contiguous")
-    bs, bst = block_table.shape, block_table.stride()
-    if len(bs) != 2 or block_table.dtype != torch.int32 or (bst[1] != 1 and bs[1] > 1):
-        raise ValueError("block_table must be [requests, blocks] int32 with contiguous rows")
-    R, W = bs
-    N = x.shape[0]
-    rps = 1
-    if cu_seqlens is None:
-        if seq_lens is None or prefix_lens is not None:
-            raise ValueError("give seq_lens, or cu_seqlens and prefix_lens")
-        if R:
-            rps = N // R
-        if seq_lens.shape != (R,) or rps * R != N:
-            raise ValueError(f"{N} rows and {tuple(seq_lens.shape)} seq_lens for {R} requests")
-        ok = seq_lens.dtype == torch.int32 and seq_lens.get_device() == dev and seq_lens.is_contiguous()
-        sl, cu, pl = seq_lens.data_ptr(), None, None
-        if N == 0:
-            R, rps = 0, 1
-    else:
-        if seq_lens is not None or prefix_lens is None:
-            raise ValueError("give seq_lens, or cu_seqlens and prefix_lens")
-        if cu_seqlens.shape != (R + 1,) or prefix_lens.shape != (R,):
-            raise ValueError(f"cu_seqlens must be [{R + 1}] and prefix_lens [{R}]")
-        ok = (cu_seqlens.dtype == torch.int32 == prefix_lens.dtype and cu_seqlens.get_device() == dev
-              and prefix_lens.get_device() == dev and cu_seqlens.is_contiguous() and prefix_lens.is_contiguous())
-        sl, cu, pl = None, cu_seqlens.data_ptr(), prefix_lens.data_ptr()
-    if not ok:
-        raise ValueError("seq_lens, cu_seqlens and prefix_lens must be contiguous int32 tensors on the rows' device")
-    if not (k_cache.get_device() == dev == v_cache.get_device() and k_scale.get_device() == dev == v_scale.get_device()
-            and block_table.get_device() == dev):
-        raise ValueError("all tensors must be on one device")
-    return R, Hkv, D, P, W, BS, rps, real, code, st, ss[0], bst[0], sl, cu, pl
-
-
+# The checks of these calls, their outputs and workspaces are the binding's
+# (csrc/bind.cpp): a decode step makes them once per layer.
 def cache8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=None, *, cu_seqlens=None,
                   prefix_lens=None):
     """Quantises new tokens k, v [N, Hkv, D] (fp32 / bf16 / fp16) into the
     pages of a scaled 8-bit cache, in place: caches [P, BS, Hkv, D]
     (float8_e4m3fn or int8; any strides with D contiguous), scales [P, Hkv]
-    fp32.  Either the last N / R tokens of each request (seq_lens [R] counts
-    them already), or varlen rows: request r's tokens are rows cu_seqlens[r]
-    .. cu_seqlens[r + 1] - 1, after prefix_lens[r] earlier ones.  Scales are
-    powers of two; a page's scale grows when new tokens need it, and its
-    earlier codes are rounded to the new scale (srswa_cache8_append)."""
-    R, Hkv, D, P, W, BS, rps, real, code, st, s_sc, s_bt, sl, cu, pl = _cache8_args(
-        k, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens)
-    N = k.shape[0]
-    if k.shape != (N, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype or v.get_device() != k.get_device():
-        raise ValueError(f"k and v must be [rows, {Hkv}, {D}] of one type on one device")
-    ks, vs = k.stride(), v.stride()
-    if ks[2] != 1:
-        k = k.contiguous()
-        ks = k.stride()
-    if vs[2] != 1:
-        v = v.contiguous()
-        vs = v.stride()
-    d = _DESC8(N, R, Hkv, Hkv, D, P, W, BS, rps, -1, 0, 0, 0.0, real, code, real, 0, ks[0], ks[1], vs[0], vs[1],
-               st[0], st[1], st[2], s_sc, s_bt, 0, 0, 0, 0, 0)
-    rc = L.lib().srswa_cache8_append(d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                     k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), sl, cu, pl,
-                                     L.stream_of(k))
-    if rc:
-        L.check(rc, "srswa_cache8_append")
+    fp32.  Either the last N / R tokens of each request (seq_lens [R] int32
+    counts them already), or varlen rows: request r's tokens are rows
+    cu_seqlens[r] .. cu_seqlens[r + 1] - 1, after prefix_lens[r] earlier ones.
+    Scales are powers of two; a page's scale grows when new tokens need it,
+    and its earlier codes are rounded to the new scale (srswa_cache8_append)."""
+    L.bind().append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens)
 
 
 def cache8_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=None, *, cu_seqlens=None,
@@ -944,173 +868,33 @@ def cache8_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=N
     (q's type, or the given out's: q's or fp32), with lse=True also the fp32
     log-sum-exp [N, H]; a row that sees nothing gives 0 and -inf.  nsplit: the
     parts the keys of a row are cut into (0: chosen)."""
-    R, Hkv, D, P, W, BS, rps, real, code, st, s_sc, s_bt, sl, cu, pl = _cache8_args(
-        q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens)
-    if real == L.F32:
-        raise NotImplementedError("q must be bfloat16 or float16")
-    shape = q.shape
-    if len(shape) != 3 or shape[2] != D or shape[1] % Hkv or shape[1] == 0:
-        raise ValueError(f"q {tuple(shape)} does not fit {Hkv} kv heads of {D}")
-    N, H, _ = shape
-    dev = q.device
-    qs = q.stride()
-    if qs[2] != 1:
-        q = q.contiguous()
-        qs = q.stride()
-    out_type = real
-    if out is None:
-        out = torch.empty_like(q)  # q's order of rows and heads, if it has no gaps
-        os_ = out.stride()
-    else:
-        if out.shape != shape or out.device != dev or out.stride(2) != 1 or out.dtype not in (q.dtype, torch.float32):
-            raise ValueError(f"out must be {tuple(shape)} of q's type or fp32, features contiguous, on {dev}")
-        os_, out_type = out.stride(), _REALS[out.dtype]
-    lse_t = torch.empty_strided((N, H), (H, 1), device=dev, dtype=torch.float32) if lse else None
-    if window is None:
-        window = -1
-    elif window < 0:
-        raise ValueError("window must be None or >= 0")
-    K = is64 = s_tn = s_th = s_bn = s_bh = 0
-    ti = bi = None
-    if topk_idx is not None:
-        ts = topk_idx.shape
-        is64 = 1 if topk_idx.dtype == torch.int64 else 0
-        if not is64 and topk_idx.dtype != torch.int32:
-            raise NotImplementedError("topk_idx must be int32 or int64")
-        if len(ts) not in (2, 3) or ts[-2] != N or (len(ts) == 3 and ts[0] not in (1, Hkv)):
-            raise ValueError(f"topk_idx {tuple(ts)} must be [{N}, K] or [{Hkv}, {N}, K]")
-        if bias is not None and (bias.shape != ts or bias.dtype != torch.float32):
-            raise ValueError("bias must be fp32 of topk_idx's shape")
-        if topk_idx.device != dev or (bias is not None and bias.device != dev):
-            raise ValueError("all tensors must be on one device")
-        ss = topk_idx.stride()
-        if ss[-1] != 1:
-            topk_idx = topk_idx.contiguous()
-            ss = topk_idx.stride()
-        heads = len(ts) == 3 and ts[0] > 1
-        K, s_tn, s_th, ti = ts[-1], ss[-2], ss[0] if heads else 0, topk_idx.data_ptr()
-        if bias is not None:
-            ss = bias.stride()
-            if ss[-1] != 1:
-                bias = bias.contiguous()
-                ss = bias.stride()
-            s_bn, s_bh, bi = ss[-2], ss[0] if heads else 0, bias.data_ptr()
-    elif bias is not None:
-        raise ValueError("bias without topk_idx")
-    d = _DESC8(N, R, H, Hkv, D, P, W, BS, rps, window, sinks, K, D ** -0.5 if sm_scale is None else sm_scale, real, code,
-               out_type, is64, qs[0], qs[1], os_[0], os_[1], st[0], st[1], st[2], s_sc, s_bt, s_th, s_tn, s_bh, s_bn,
-               nsplit)
-    lib = L.lib()
-    need = lib.srswa_cache8_attend_workspace_size(d, 0 if cu is None else 1)
-    ws = None
-    if need:
-        ws = (torch.empty_strided((need,), (1,), device=dev, dtype=torch.uint8) if workspace is None
-              else _workspace(need, dev, workspace)).data_ptr()
-    rc = lib.srswa_cache8_attend(d, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                                 v_scale.data_ptr(), block_table.data_ptr(), sl, cu, pl, ti, bi, out.data_ptr(),
-                                 L.ptr(lse_t), ws, need, L.stream_of(q))
-    if rc:
-        L.check(rc, "srswa_cache8_attend")
-    return (out, lse_t) if lse else out
+    return L.bind().attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens, window,
+                           sinks, topk_idx, bias, sm_scale, out, lse, nsplit, workspace)
 
 
 # ------------------------------------------------------- pages of a cache
-def _page_args(block_table, seq_lens, refs, *rows):
-    bs, st, dev = block_table.shape, block_table.stride(), block_table.get_device()
-    if len(bs) != 2 or block_table.dtype != torch.int32 or (st[1] != 1 and bs[1] > 1):
-        raise ValueError("block_table must be [rows, blocks] int32 with contiguous rows")
-    if seq_lens is not None:
-        if seq_lens.shape != (bs[0],):
-            raise ValueError("seq_lens must be [rows]")
-        rows += (seq_lens,)
-    for t in (refs, *rows):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
-            raise ValueError("row lists, seq_lens and refs must be contiguous int32 tensors on the table's device")
-    return block_table.data_ptr(), st[0], bs[0], bs[1], refs.shape[0]
-
-
-def _page_tensors(tensors, P, dev):
-    """srswa_page_tensor array of tensors [P, ...] whose pages are each one
-    run of bytes (the other dimensions in any order, none padded)."""
-    words = []
-    for i, t in enumerate(tensors):
-        shape, st = t.shape, t.stride()
-        if len(shape) == 0 or shape[0] != P or t.get_device() != dev:
-            raise ValueError(f"tensor {i}: {tuple(shape)} is not indexed by {P} pages on the table's device")
-        if t.is_contiguous() or (len(shape) == 4 and st[3] == 1 and st[1] == shape[3] and st[2] == shape[1] * shape[3]
-                                 and st[0] == shape[2] * st[2]):  # (page, head) tiles
-            n = step = t.nbytes // P if P else 0
-        else:
-            es = t.element_size()
-            n = 1
-            for size, stride in sorted(zip(shape[1:], st[1:]), key=lambda x: x[1]):
-                if size != 1 and stride != n:
-                    raise ValueError(f"tensor {i}: a page must be one run of elements, got {tuple(shape)} "
-                                     f"with strides {st}")
-                n *= size
-            if P > 1 and st[0] < n:
-                raise ValueError(f"tensor {i}: pages overlap: {tuple(shape)} with strides {st}")
-            n, step = n * es, max(st[0], n) * es
-        words += (t.data_ptr(), n, step)
-    return struct.pack(f"@{len(words)}q", *words) if words else None
-
-
-def _page_scratch(n, dev):
-    """A one-element result and n ints of scratch (empty_strided: the cheapest
-    way to them, a microsecond less each than empty)."""
-    return (torch.empty_strided((1,), (1,), device=dev, dtype=torch.int32),
-            torch.empty_strided((n,), (1,), device=dev, dtype=torch.int32))
-
-
 def pages_free(rows, block_table, seq_lens, refs, *, block_size):
     """Gives up the pages of table rows ``rows`` (int32 ids; those outside the
     table and repeats do nothing): counts down, entries -1, lengths 0, in
     place.  block_table [R, W], seq_lens [R] (tokens), refs [P] (table entries
     naming each page), all int32."""
-    bt, s_bt, R, W, P = _page_args(block_table, seq_lens, refs, rows)
-    rc = L.lib().srswa_pages_free(rows.data_ptr(), rows.shape[0], bt, s_bt, R, W, seq_lens.data_ptr(),
-                                  refs.data_ptr(), P, block_size, L.stream_of(block_table))
-    if rc:
-        L.check(rc, "srswa_pages_free")
+    L.bind().pages_free(rows, block_table, seq_lens, refs, block_size)
 
 
 def pages_extend(rows, new_lens, block_table, seq_lens, refs, *, block_size):
     """Grows table rows ``rows`` to ``new_lens`` tokens with the lowest free
     pages, rows served in order, in place (srswa_pages_extend).  Returns an
     int32 [1] device tensor: rows left as they were for lack of pages."""
-    bt, s_bt, R, W, P = _page_args(block_table, seq_lens, refs, rows, new_lens)
-    n = rows.shape[0]
-    if new_lens.shape[0] != n:
-        raise ValueError("rows and new_lens must be equally long")
-    stream = L.stream_of(block_table)
-    short, ws = _page_scratch(n + R + P, rows.device)
-    rc = L.lib().srswa_pages_extend(rows.data_ptr(), new_lens.data_ptr(), n, bt, s_bt, R, W, seq_lens.data_ptr(),
-                                    refs.data_ptr(), P, block_size, short.data_ptr(), ws.data_ptr(), 4 * (n + R + P),
-                                    stream)
-    if rc:
-        L.check(rc, "srswa_pages_extend")
-    return short
+    return L.bind().pages_extend(rows, new_lens, block_table, seq_lens, refs, block_size)
 
 
 def pages_fork(parents, children, block_table, seq_lens, refs, tensors, *, block_size):
     """Makes each empty table row children[i] a copy of row parents[i], in
     place: full pages are shared, a part-filled last page is copied, in every
-    tensor of ``tensors`` ([P, ...]), into the lowest free page
-    (srswa_pages_fork).  Returns an int32 [1] device tensor: children not made
-    for lack of pages."""
-    bt, s_bt, R, W, P = _page_args(block_table, seq_lens, refs, parents, children)
-    n = parents.shape[0]
-    if children.shape[0] != n:
-        raise ValueError("parents and children must be equally long")
-    arr = _page_tensors(tensors, P, block_table.get_device())
-    stream = L.stream_of(block_table)
-    short, ws = _page_scratch(n + R + P, parents.device)
-    rc = L.lib().srswa_pages_fork(parents.data_ptr(), children.data_ptr(), n, bt, s_bt, R, W, seq_lens.data_ptr(),
-                                  refs.data_ptr(), P, block_size, arr, len(tensors), short.data_ptr(), ws.data_ptr(),
-                                  4 * (n + R + P), stream)
-    if rc:
-        L.check(rc, "srswa_pages_fork")
-    return short
+    tensor of ``tensors`` ([P, ...], the bytes of a page in one run), into the
+    lowest free page (srswa_pages_fork).  Returns an int32 [1] device tensor:
+    children not made for lack of pages."""
+    return L.bind().pages_fork(parents, children, block_table, seq_lens, refs, tensors, block_size)
 
 
 def pages_compact(block_table, refs, tensors, *, out_table=None, out_refs=None):
@@ -1119,24 +903,4 @@ def pages_compact(block_table, refs, tensors, *, out_table=None, out_refs=None):
     counts afterwards (new tensors, or out_table / out_refs, which may be the
     inputs themselves) and an int32 [1] device tensor, the pages in use
     (srswa_pages_compact)."""
-    bt, s_bt, R, W, P = _page_args(block_table, None, refs)
-    dev = block_table.device
-    if out_table is None:
-        out_table = torch.empty_strided((R, W), (W, 1), device=dev, dtype=torch.int32)
-    elif (out_table.shape != (R, W) or out_table.dtype != torch.int32 or out_table.device != dev
-          or (out_table.stride(1) != 1 and W > 1)):
-        raise ValueError(f"out_table must be {(R, W)} int32 with contiguous rows on {dev}")
-    if out_refs is None:
-        out_refs = torch.empty_like(refs)
-    elif out_refs.shape != (P,) or out_refs.dtype != torch.int32 or not out_refs.is_contiguous() or out_refs.device != dev:
-        raise ValueError(f"out_refs must be contiguous int32 [{P}] on {dev}")
-    arr = _page_tensors(tensors, P, block_table.get_device())
-    stream = L.stream_of(block_table)
-    lib = L.lib()
-    need = lib.srswa_pages_compact_workspace_size(P)
-    live, ws = _page_scratch(need // 4, dev)
-    rc = lib.srswa_pages_compact(bt, s_bt, R, W, refs.data_ptr(), P, arr, len(tensors), out_table.data_ptr(),
-                                 out_table.stride(0), out_refs.data_ptr(), live.data_ptr(), ws.data_ptr(), need, stream)
-    if rc:
-        L.check(rc, "srswa_pages_compact")
-    return out_table, out_refs, live
+    return L.bind().pages_compact(block_table, refs, tensors, out_table, out_refs)
