@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const 
   constexpr int TPP = kAppendThreads / LPT;      // tokens per pass
   constexpr int NP = 8;                          // passes held in registers
   __shared__ float red[kAppendThreads / 32];
+  pdl_launch_dependents();
+  pdl_wait();
   const int tid = threadIdx.x;
   const int64_t head = blockIdx.y;
   const int which = blockIdx.z;
@@ -250,6 +252,8 @@ __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const 
 template <int D, int KVT>
 __global__ void __launch_bounds__(kAppendThreads) cache8_append_one_kernel(const AppendArgs a) {
   constexpr int E = D / 32;
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int which = static_cast<int>(item % 2);
@@ -286,14 +290,13 @@ __global__ void __launch_bounds__(kAppendThreads) cache8_append_one_kernel(const
 }
 
 template <int D, int KVT>
-static void append_start(const AppendArgs& a, int64_t slots, cudaStream_t st) {
+static int append_start(const AppendArgs& a, int64_t slots, cudaStream_t st) {
   if (!a.rows.cu && a.rows.rps == 1) {
     const int64_t ctas = (2 * a.rows.R * a.Hkv + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-    cache8_append_one_kernel<D, KVT><<<static_cast<unsigned>(ctas), kAppendThreads, 0, st>>>(a);
-  } else {
-    const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(a.Hkv), 2);
-    cache8_append_kernel<D, KVT><<<grid, kAppendThreads, 0, st>>>(a);
+    return launch_pdl(cache8_append_one_kernel<D, KVT>, dim3(static_cast<unsigned>(ctas)), kAppendThreads, 0, st, a);
   }
+  const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(a.Hkv), 2);
+  return launch_pdl(cache8_append_kernel<D, KVT>, grid, kAppendThreads, 0, st, a);
 }
 
 }  // namespace srswa
@@ -351,14 +354,9 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
   a.s_page = d->s_page; a.s_pos = d->s_pos; a.s_head = d->s_head; a.s_scale = d->s_scale;
   a.x_dtype = d->q_dtype;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (d->D == 128) {
-    if (d->kv_dtype == SRSWA_I8) append_start<128, SRSWA_I8>(a, slots, st);
-    else append_start<128, SRSWA_F8E4M3>(a, slots, st);
-  } else {
-    if (d->kv_dtype == SRSWA_I8) append_start<64, SRSWA_I8>(a, slots, st);
-    else append_start<64, SRSWA_F8E4M3>(a, slots, st);
-  }
-  return srswa_last_launch_status();
+  if (d->D == 128)
+    return d->kv_dtype == SRSWA_I8 ? append_start<128, SRSWA_I8>(a, slots, st) : append_start<128, SRSWA_F8E4M3>(a, slots, st);
+  return d->kv_dtype == SRSWA_I8 ? append_start<64, SRSWA_I8>(a, slots, st) : append_start<64, SRSWA_F8E4M3>(a, slots, st);
 }
 
 extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen) {

@@ -40,6 +40,7 @@ constexpr int kRowsThreads = 128;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsRing = 16384;  // shared memory of a warp's ring at D = 128 (half of it at 64)
 constexpr int kRowsCtasPerSm = 3;
+constexpr int kRowsCtaWarps = 6;  // of a CTA whose warps share an item, where there is room for two on each SM
 #ifndef PREFER_CH
 #define PREFER_CH 2
 #endif
@@ -112,8 +113,8 @@ __device__ __forceinline__ uint32_t v_off(int r, int c) {
 // CH: 16-key chunks of a unit, what a warp takes at a time (a divisor of a
 // page's chunks; two amortise the softmax bookkeeping and keep two independent
 // MMA chains going).
-template <int D, int KVT, int CH, bool MULTI>
-__global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kernel(const Attend8Args a) {
+template <int D, int KVT, int CH, bool MULTI, int NW>
+__global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cache8_rows_kernel(const Attend8Args a) {
   constexpr int CB = 16 * D;           // bytes of a chunk of K (or V)
   constexpr int SB = 2 * CH * CB;      // bytes of a stage: K of its chunks, then V
   constexpr int ST = kRowsRing * D / 128 / SB;  // stages of a warp's ring
@@ -121,8 +122,8 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   constexpr int KS = D / 16;           // MMA steps of a dot product, and feature tiles of the output
   constexpr int RPI = 512 / D;         // key rows per warp copy instruction
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t f_sum[kRowsThreads + 1];
-  __shared__ float w_ml[kRowsWarps][2 * kCols];
+  __shared__ int64_t f_sum[(32 * NW) + 1];
+  __shared__ float w_ml[NW][2 * kCols];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
@@ -134,7 +135,8 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   const uint32_t ring = smem_u32(smem) + warp * ST * SB;
   const int krow = (g >> 1) + 4 * (g & 1);  // the key of MMA row g (and + 8 of row g + 8)
   const int cr = lane / (D / 16), cc = lane % (D / 16);  // key row and 16-byte unit of this lane's copies
-  pdl_launch_dependents();                  // the merge kernel waits for this grid before it reads
+  pdl_launch_dependents();
+  pdl_wait();
 
   // One (row group, kv head, column group), units [c0, c1) of its `s.units`.
   // po == nullptr: the whole item, results written out; else a part: its
@@ -485,15 +487,15 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
   };
 
   const int64_t per_group = a.Hkv * a.ngrp;  // items of a row group
-  const int64_t me = static_cast<int64_t>(blockIdx.x) * kRowsWarps + warp;  // this warp's part
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * NW + warp;  // this warp's part
   const int64_t groups = a.N / share;
   int64_t req, pos, stop, rg, off;
   Span s;
   if (a.split == kSplitCta) {  // a quarter of the CTA's item
     rg = blockIdx.x / per_group;
     s = group_span<CH>(a, rg, req);
-    pos = s.units * warp / kRowsWarps;
-    stop = s.units * (warp + 1) / kRowsWarps;
+    pos = s.units * warp / NW;
+    stop = s.units * (warp + 1) / NW;
     off = (blockIdx.x % per_group) * s.units + pos;
   } else if (a.split == kSplitNone) {  // one warp per item
     rg = me / per_group;
@@ -503,7 +505,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
     stop = s.units;
     off = (me % per_group) * s.units;
   } else {  // an equal part of all units
-    const int64_t per = (groups + kRowsThreads - 1) / kRowsThreads;
+    const int64_t per = (groups + (32 * NW) - 1) / (32 * NW);
     const int64_t g_lo = min(tid * per, groups), g_hi = min(g_lo + per, groups);
     int64_t sum = 0;
     for (int64_t i = g_lo; i < g_hi; ++i) sum += group_span<CH>(a, i, req).units;
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
     if (warp == 0) {  // prefix sums of the threads' shares
       int64_t run = 0;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
+      for (int w = 0; w < NW; ++w) {
         int64_t x = f_sum[w * 32 + lane + 1];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -525,11 +527,11 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
       }
     }
     __syncthreads();
-    const int64_t total = f_sum[kRowsThreads] * per_group, parts = static_cast<int64_t>(gridDim.x) * kRowsWarps;
+    const int64_t total = f_sum[(32 * NW)] * per_group, parts = static_cast<int64_t>(gridDim.x) * NW;
     pos = total * me / parts;
     stop = total * (me + 1) / parts;
     // the share, then the row group, that holds unit `pos`
-    int lo = 0, hi = kRowsThreads;
+    int lo = 0, hi = (32 * NW);
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (f_sum[mid] * per_group <= pos) lo = mid;
@@ -578,15 +580,15 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtasPerSm) cache8_rows_kern
     __syncthreads();
     const int64_t it = blockIdx.x % per_group, hk = it / a.ngrp, row0 = blockIdx.x / per_group * share;
     const int first = static_cast<int>(it % a.ngrp) * kCols, ncol = min(share * G - first, kCols);
-    for (int i = tid; i < ncol * D; i += kRowsThreads) {
+    for (int i = tid; i < ncol * D; i += (32 * NW)) {
       const int col = i / D, d = i % D, gc = first + col;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, w_ml[w][2 * col]);
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, w_ml[w][2 * col]);
       const float Mu = M == -INFINITY ? 0.f : M;
       float L = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = exp2f(w_ml[w][2 * col] - Mu);
         L += w_ml[w][2 * col + 1] * f;
         x += reinterpret_cast<const float*>(smem + w * ST * SB)[col * D + d] * f;
@@ -606,6 +608,8 @@ template <int D>
 __global__ void __launch_bounds__(128) cache8_merge_kernel(const Attend8Args a, int parts) {
   constexpr int V = D / 32;  // features of a lane
   __shared__ float wt[128], red[4][D], top[4];
+  // (no early launch of what follows: beside these CTAs a next attend would not fit
+  // three to an SM, and its equal parts want to start together: 171 us for 130)
   pdl_wait();
   const int c = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int4* meta = reinterpret_cast<const int4*>(a.part_meta);
@@ -701,15 +705,17 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   const int64_t most = (blocks + d.K) * upp;
   const int64_t slots = static_cast<int64_t>(sm_count()) * kRowsCtasPerSm * kRowsWarps;
   int64_t parts = p.items;
+  p.warps = kRowsWarps;
   p.split = kSplitNone;
   if (d.nsplit > 0) {
     if (d.nsplit > 1) p.split = kSplitEqual;
     parts = d.nsplit * p.items;
   } else if (p.items <= slots / kRowsWarps && most <= 16 * kRowsWarps) {
-    // one wave of CTAs, at most 16 units a warp: 10 items of 9 units take TIME1 us
-    // against TIME2 with equal parts and a join, 288 of up to 35 TIME3 against TIME4
+    // one wave of CTAs, at most 16 units a warp (measured: the table of
+    // cache8_rows_kernel)
     p.split = kSplitCta;
-    parts = p.items * kRowsWarps;
+    if (p.items <= slots / kRowsCtaWarps) p.warps = kRowsCtaWarps;
+    parts = p.items * p.warps;
   } else if (most <= 2 || groups > 2048 || p.items > 16 * slots || (p.items >= slots && most <= 16)) {
     // items that a warp is through with at once, or so many that their uneven
     // ends do not show: one warp each, no join
@@ -718,7 +724,7 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
     const int64_t enough = (p.items * most + 1) / 2;  // two units each at least
     parts = enough < slots ? enough : slots;
   }
-  p.ctas = (parts + kRowsWarps - 1) / kRowsWarps;
+  p.ctas = (parts + p.warps - 1) / p.warps;
   if (p.split == kSplitEqual) {
     parts = p.ctas * kRowsWarps;
     const int64_t f = parts * 2 * kCols;
@@ -728,9 +734,10 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   return p;
 }
 
-template <int D, int KVT, int CH, bool MULTI>
-static int rows_start(const Attend8Args& a, unsigned ctas, int ring, cudaStream_t st) {
-  auto kern = cache8_rows_kernel<D, KVT, CH, MULTI>;
+template <int D, int KVT, int CH, bool MULTI, int NW>
+static int rows_start(const Attend8Args& a, unsigned ctas, cudaStream_t st) {
+  auto kern = cache8_rows_kernel<D, KVT, CH, MULTI, NW>;
+  const int ring = NW * kRowsRing * D / 128;
   static bool allowed[64] = {};  // per device: the shared memory has been asked for
   int dev = 0;
   SRSWA_CUDA_TRY(cudaGetDevice(&dev));
@@ -738,8 +745,7 @@ static int rows_start(const Attend8Args& a, unsigned ctas, int ring, cudaStream_
     SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
     if (dev < 64) allowed[dev] = true;
   }
-  kern<<<ctas, kRowsThreads, ring, st>>>(a);
-  return srswa_last_launch_status();
+  return launch_pdl(kern, dim3(ctas), 32 * NW, ring, st, a);
 }
 
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st) {
@@ -751,15 +757,19 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   a.part_ml = a.part_o + p.o_floats;
   const int64_t parts = p.ctas * kRowsWarps;
   a.part_meta = reinterpret_cast<int*>(a.part_ml + parts * 2 * kCols * 2);
-  const int ring = kRowsWarps * kRowsRing * static_cast<int>(a.D) / 128;
   const unsigned ctas = static_cast<unsigned>(p.ctas);
+  auto by_warps = [&](auto d_, auto ch_, auto type_, auto multi_) -> int {
+    constexpr int D = decltype(d_)::value, CH = decltype(ch_)::value, KVT = decltype(type_)::value;
+    constexpr bool MULTI = decltype(multi_)::value;
+    return p.warps == kRowsWarps ? rows_start<D, KVT, CH, MULTI, kRowsWarps>(a, ctas, st)
+                                 : rows_start<D, KVT, CH, MULTI, kRowsCtaWarps>(a, ctas, st);
+  };
   auto by_type = [&](auto d_, auto ch_) -> int {
-    constexpr int D = decltype(d_)::value, CH = decltype(ch_)::value;
+    using I8 = std::integral_constant<int, SRSWA_I8>;
+    using E4 = std::integral_constant<int, SRSWA_F8E4M3>;
     if (p.share > 1)
-      return kv_dtype == SRSWA_I8 ? rows_start<D, SRSWA_I8, CH, true>(a, ctas, ring, st)
-                                  : rows_start<D, SRSWA_F8E4M3, CH, true>(a, ctas, ring, st);
-    return kv_dtype == SRSWA_I8 ? rows_start<D, SRSWA_I8, CH, false>(a, ctas, ring, st)
-                                : rows_start<D, SRSWA_F8E4M3, CH, false>(a, ctas, ring, st);
+      return kv_dtype == SRSWA_I8 ? by_warps(d_, ch_, I8(), std::true_type()) : by_warps(d_, ch_, E4(), std::true_type());
+    return kv_dtype == SRSWA_I8 ? by_warps(d_, ch_, I8(), std::false_type()) : by_warps(d_, ch_, E4(), std::false_type());
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
@@ -768,18 +778,10 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   const int rc = a.D == 128 ? (p.ch == 2 ? by_type(D128(), Two()) : by_type(D128(), One()))
                             : (p.ch == 2 ? by_type(D64(), Two()) : by_type(D64(), One()));
   if (rc || p.split != kSplitEqual) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(parts), static_cast<unsigned>(p.share * (a.H / a.Hkv) < kCols ? p.share * (a.H / a.Hkv) : kCols), 1);
-  cfg.blockDim = dim3(128, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = a.D == 128 ? cudaLaunchKernelEx(&cfg, cache8_merge_kernel<128>, a, static_cast<int>(parts))
-                                   : cudaLaunchKernelEx(&cfg, cache8_merge_kernel<64>, a, static_cast<int>(parts));
-  return e == cudaSuccess ? 0 : static_cast<int>(e);
+  const int64_t cols = p.share * (a.H / a.Hkv);
+  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(cols < kCols ? cols : kCols));
+  return a.D == 128 ? launch_pdl(cache8_merge_kernel<128>, grid, 128, 0, st, a, static_cast<int>(parts))
+                    : launch_pdl(cache8_merge_kernel<64>, grid, 128, 0, st, a, static_cast<int>(parts));
 }
 
 }  // namespace srswa

@@ -73,7 +73,8 @@ struct RowsPlan {
   int64_t share, ngrp, items, ctas, o_floats;
   size_t bytes;  // workspace
   int split;
-  int ch;  // 16-key chunks of a unit
+  int ch;     // 16-key chunks of a unit
+  int warps;  // of a CTA
 };
 RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen);
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st);

@@ -202,6 +202,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = static_cast<int>(a.H / a.Hkv);
   const int64_t hk = blockIdx.y;
+  pdl_launch_dependents();
+  pdl_wait();
   PrTile T;
   // the last tiles of a prompt have the most keys: they go first
   if (!T.set(a, gridDim.x - 1 - blockIdx.x, G)) return;
@@ -688,8 +690,7 @@ int prompt_launch(const Attend8Args& a, int kv_dtype, int* status, cudaStream_t 
       SRSWA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
       if (dev < 64) allowed[dev] = true;
     }
-    kern<<<grid, kPrThreads, smem, st>>>(a, status);
-    return srswa_last_launch_status();
+    return launch_pdl(kern, grid, kPrThreads, smem, st, a, status);
   };
   static bool allowed[4][64] = {};  // per kernel and device: the shared memory has been asked for
   if (a.D == 128) {

@@ -180,3 +180,23 @@ static inline int srswa_last_launch_status() {
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
+
+namespace srswa {
+// Launch that may begin while the kernel ahead on the stream runs: the kernel
+// executes pdl_wait() before it reads or writes anything.
+template <typename... P, typename... A>
+static int launch_pdl(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? 0 : static_cast<int>(e);
+}
+}  // namespace srswa

@@ -73,10 +73,12 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total) {
   return before + x - v;
 }
 
-__global__ void __launch_bounds__(256) pages_free_kernel(const int32_t* __restrict__ rows, int32_t* table, int64_t s_bt,
+__global__ void __launch_bounds__(256) pages_free_kernel(const int32_t* rows, int32_t* table, int64_t s_bt,
                                                          int64_t R, int64_t W, int32_t* seq_lens, int32_t* refs,
                                                          int64_t P, int64_t BS) {
   __shared__ int len;
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t row = rows[blockIdx.x];
   if (row < 0 || row >= R) return;
   // a row named twice: whoever takes its length first does the work
@@ -129,6 +131,7 @@ __device__ __forceinline__ bool plan_item(const PlanArgs& a, int64_t i, int64_t&
 __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanArgs a) {
   const int tid = threadIdx.x;
   pdl_launch_dependents();
+  pdl_wait();
   for (int64_t i = tid; i < a.n; i += kPlanThreads) {
     int64_t row, need;
     if (plan_item(a, i, row, need)) a.claim[row] = 0x7fffffff;
@@ -177,6 +180,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanArgs
 }
 
 __global__ void __launch_bounds__(256) pages_extend_kernel(const PlanArgs a) {
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t i = blockIdx.x;
   const int64_t at = a.first[i];
@@ -195,6 +199,7 @@ __global__ void __launch_bounds__(256) pages_extend_kernel(const PlanArgs a) {
 // grid (1 + chunks of a page, items): part 0 makes the child's row, the others
 // copy the part-filled page.
 __global__ void __launch_bounds__(256) pages_fork_kernel(const PlanArgs a, const PageTensors pt) {
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t i = blockIdx.y;
   const int64_t at = a.first[i];
@@ -240,6 +245,7 @@ struct CompactArgs {
 __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const CompactArgs a) {
   const int tid = threadIdx.x;
   pdl_launch_dependents();
+  pdl_wait();
   int64_t mine = 0, live;
   for (int64_t p = tid; p < a.P; p += kPlanThreads) mine += a.refs[p] > 0;
   block_scan(mine, live);
@@ -274,6 +280,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
 }
 
 __global__ void __launch_bounds__(256) pages_compact_kernel(const CompactArgs a, const PageTensors pt) {
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t work = static_cast<int64_t>(*a.moves) * pt.chunks;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
@@ -287,22 +294,6 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(const CompactArgs a,
     const int32_t p = a.table[r * a.s_bt + b];
     a.out_table[r * a.s_out + b] = p >= 0 && p < a.P ? a.to[p] : p;
   }
-}
-
-template <typename... P, typename... A>
-static int launch_after(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
-  // may start while the plan kernel runs: it waits for it before reading anything
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
 
 }  // namespace srswa
@@ -345,8 +336,7 @@ static int make_plan(PlanArgs& a, void* workspace, size_t workspace_bytes, cudaS
   a.claim = static_cast<int32_t*>(workspace);
   a.first = a.claim + a.R;
   a.pages = a.first + a.n;
-  pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
-  return srswa_last_launch_status();
+  return launch_pdl(pages_plan_kernel, dim3(1), kPlanThreads, 0, st, a);
 }
 
 extern "C" int srswa_pages_free(const int32_t* rows, int64_t n, int32_t* block_table, int64_t s_bt, int64_t R,
@@ -357,9 +347,8 @@ extern "C" int srswa_pages_free(const int32_t* rows, int64_t n, int32_t* block_t
   SRSWA_CHECK_ARG(n >= 0 && block_size > 0 && seq_lens && (n == 0 || rows), SRSWA_EINVAL);
   SRSWA_CHECK_ARG(n < (1ll << 31), SRSWA_ETOOLARGE);
   if (n == 0) return SRSWA_OK;
-  pages_free_kernel<<<static_cast<unsigned>(n), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      rows, block_table, s_bt, R, W, seq_lens, refs, P, block_size);
-  return srswa_last_launch_status();
+  return launch_pdl(pages_free_kernel, dim3(static_cast<unsigned>(n)), 256, 0, reinterpret_cast<cudaStream_t>(stream),
+                    rows, block_table, s_bt, R, W, seq_lens, refs, P, block_size);
 }
 
 extern "C" int srswa_pages_extend(const int32_t* rows, const int32_t* new_lens, int64_t n, int32_t* block_table,
@@ -374,7 +363,7 @@ extern "C" int srswa_pages_extend(const int32_t* rows, const int32_t* new_lens, 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = make_plan(a, workspace, workspace_bytes, st);
   if (rc || n == 0) return rc;
-  return launch_after(pages_extend_kernel, dim3(static_cast<unsigned>(n)), 256, st, a);
+  return launch_pdl(pages_extend_kernel, dim3(static_cast<unsigned>(n)), 256, 0, st, a);
 }
 
 extern "C" int srswa_pages_fork(const int32_t* parents, const int32_t* children, int64_t n, int32_t* block_table,
@@ -392,8 +381,8 @@ extern "C" int srswa_pages_fork(const int32_t* parents, const int32_t* children,
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = make_plan(a, workspace, workspace_bytes, st);
   if (rc || n == 0) return rc;
-  return launch_after(pages_fork_kernel, dim3(static_cast<unsigned>(1 + pt.chunks), static_cast<unsigned>(n)), 256, st,
-                      a, pt);
+  return launch_pdl(pages_fork_kernel, dim3(static_cast<unsigned>(1 + pt.chunks), static_cast<unsigned>(n)), 256, 0, st,
+                    a, pt);
 }
 
 extern "C" size_t srswa_pages_compact_workspace_size(int64_t P) {
@@ -419,8 +408,7 @@ extern "C" int srswa_pages_compact(const int32_t* block_table, int64_t s_bt, int
   a.dst = a.src + P;
   a.to = a.dst + P;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  pages_compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
-  rc = srswa_last_launch_status();
+  rc = launch_pdl(pages_compact_plan_kernel, dim3(1), kPlanThreads, 0, st, a);
   if (rc) return rc;
-  return launch_after(pages_compact_kernel, dim3(148 * 8), 256, st, a, pt);
+  return launch_pdl(pages_compact_kernel, dim3(148 * 8), 256, 0, st, a, pt);
 }
