@@ -790,7 +790,7 @@ typedef struct {
 } srswa_page_tensor;
 enum { SRSWA_MAX_PAGE_TENSORS = 16 };
 
-/* int32 scratch of the three calls below for n items. */
+/* Bytes of scratch (16-byte aligned) of extend and fork for n items. */
 SRSWA_API size_t srswa_pages_workspace_size(int64_t n, int64_t R, int64_t P);
 
 /* Gives up the pages of rows[i] (n row ids; ids outside [0, R) and repeats do

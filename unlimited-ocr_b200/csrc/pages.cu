@@ -24,7 +24,7 @@ struct PageTensors {
   } t[SRSWA_MAX_PAGE_TENSORS];
 };
 
-// One chunk of page src to page dst, by the whole CTA.
+// One chunk of page src to page dst, by the whole CTA (256 threads).
 __device__ __forceinline__ void copy_chunk(const PageTensors& pt, int chunk, int64_t src, int64_t dst) {
   int i = 0;
   while (i + 1 < pt.n && pt.t[i + 1].first <= chunk) ++i;
@@ -35,7 +35,16 @@ __device__ __forceinline__ void copy_chunk(const PageTensors& pt, int chunk, int
   if (pt.t[i].align == 16) {
     const uint4* s4 = reinterpret_cast<const uint4*>(s);
     uint4* d4 = reinterpret_cast<uint4*>(d);
-    for (int64_t e = threadIdx.x; e < n / 16; e += blockDim.x) d4[e] = s4[e];
+    // all of a thread's loads before its first store
+    constexpr int kEach = kChunkBytes / 16 / 256;
+    const int n4 = static_cast<int>(n / 16);
+    uint4 v[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (static_cast<int>(threadIdx.x) + 256 * i < n4) v[i] = s4[threadIdx.x + 256 * i];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (static_cast<int>(threadIdx.x) + 256 * i < n4) d4[threadIdx.x + 256 * i] = v[i];
   } else if (pt.t[i].align == 4) {
     const uint32_t* s4 = reinterpret_cast<const uint32_t*>(s);
     uint32_t* d4 = reinterpret_cast<uint32_t*>(d);
@@ -92,6 +101,12 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const int32_t* rows, in
   }
 }
 
+// One item as the apply kernels take it: everything they need in one read.
+struct __align__(16) PlanItem {
+  int32_t made, row, len, have;     // carried out; row that changes; its new length; pages it has
+  int32_t first, parent, src, dst;  // rank of its first free page; fork: parent row, part-filled page, its copy (-1)
+};
+
 struct PlanArgs {
   const int32_t* rows;     // fork: children; extend: rows
   const int32_t* parents;  // fork
@@ -103,52 +118,71 @@ struct PlanArgs {
   int32_t* refs;
   int32_t* short_out;
   // workspace
-  int32_t* claim;  // [R] the first item that names a row
-  int32_t* first;  // [n] rank of the item's first free page, -1: void or not made
-  int32_t* pages;  // [P] free pages, lowest first
+  PlanItem* items;  // [n]
+  int32_t* claim;   // [R] the first item that names a row (kept on chip for up to kClaimRows rows)
+  int32_t* pages;   // [P] free pages, lowest first
 };
+constexpr int kClaimRows = 8192;
 
 __device__ __forceinline__ int64_t pages_for(int64_t tokens, int64_t BS) { return (tokens + BS - 1) / BS; }
 
-// Whether item i would be carried out, apart from repeats, and the new pages it needs.
-__device__ __forceinline__ bool plan_item(const PlanArgs& a, int64_t i, int64_t& row, int64_t& need) {
+// Whether item i would be carried out, apart from repeats; its row, the new pages
+// it needs, the new length, and the pages that the row has.
+__device__ __forceinline__ bool plan_item(const PlanArgs& a, int64_t i, int64_t& row, int64_t& need, int64_t& len,
+                                          int64_t& have) {
   row = a.rows[i];
-  if (row < 0 || row >= a.R) return false;
-  const int64_t have = a.seq_lens[row];
+  const int64_t par = a.parents ? a.parents[i] : 0;
+  const int64_t want = a.lens ? a.lens[i] : 0;
+  if (row < 0 || row >= a.R || par < 0 || par >= a.R) return false;
+  const int64_t now = a.seq_lens[row];
+  len = a.parents ? a.seq_lens[par] : want;
+  have = pages_for(now, a.BS);
+  if (now < 0 || pages_for(len, a.BS) > a.W) return false;
   if (a.parents) {
-    const int64_t par = a.parents[i];
-    if (par < 0 || par >= a.R || have != 0) return false;
-    const int64_t len = a.seq_lens[par];
     need = len % a.BS ? 1 : 0;
-    return len > 0 && pages_for(len, a.BS) <= a.W;
+    return now == 0 && len > 0;
   }
-  const int64_t len = a.lens[i];
-  if (len < have || pages_for(len, a.BS) > a.W) return false;
-  need = pages_for(len, a.BS) - pages_for(have, a.BS);
-  return true;
+  need = pages_for(len, a.BS) - have;
+  return len >= now;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanArgs a) {
+  __shared__ int32_t near_claim[kClaimRows];
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
+  int32_t* claim = a.R <= kClaimRows ? near_claim : a.claim;
+  // more items than threads: they are looked at again in each pass
+  int64_t row = 0, need = 0, len = 0, have = 0;
+  bool ok = false;
+  const bool once = a.n <= kPlanThreads;
+  auto look = [&](int64_t i) { ok = i < a.n && plan_item(a, i, row, need, len, have); };
   for (int64_t i = tid; i < a.n; i += kPlanThreads) {
-    int64_t row, need;
-    if (plan_item(a, i, row, need)) a.claim[row] = 0x7fffffff;
+    look(i);
+    if (ok) claim[row] = 0x7fffffff;
   }
   __syncthreads();
   for (int64_t i = tid; i < a.n; i += kPlanThreads) {
-    int64_t row, need;
-    if (plan_item(a, i, row, need)) atomicMin(&a.claim[row], static_cast<int>(i));
+    if (!once) look(i);
+    if (ok) atomicMin(&claim[row], static_cast<int>(i));
   }
   __syncthreads();
   int64_t all = 0;  // pages the items need together
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + tid;
-    int64_t row = 0, need = 0, sum;
-    const bool ok = i < a.n && plan_item(a, i, row, need) && a.claim[row] == i;
-    const int64_t at = all + block_scan(ok ? need : 0, sum);
-    if (i < a.n) a.first[i] = ok ? static_cast<int32_t>(min(at, static_cast<int64_t>(0x7ffffffe))) : -1;
+    if (!once) look(i);
+    const bool mine = ok && claim[row] == i;
+    int64_t sum;
+    const int64_t at = all + block_scan(mine ? need : 0, sum);
+    if (i < a.n) {
+      PlanItem x = {mine ? 1 : 0, static_cast<int32_t>(row), static_cast<int32_t>(len), static_cast<int32_t>(have),
+                    static_cast<int32_t>(min(at, static_cast<int64_t>(0x7ffffffe))), 0, -1, -1};
+      if (mine && a.parents) {
+        x.parent = a.parents[i];
+        if (need) x.src = a.table[x.parent * a.s_bt + len / a.BS];
+      }
+      a.items[i] = x;
+    }
     all += sum;
   }
   // the lowest free pages, as many as are needed
@@ -165,16 +199,17 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanArgs
   int64_t miss = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + tid;
-    int64_t row, need = 0, sum;
-    const bool ok = i < a.n && a.first[i] >= 0;
     bool none = false;
-    if (ok) {
-      plan_item(a, i, row, need);
-      none = need > 0 && a.first[i] + need > found;
-      if (none) a.first[i] = -1;
+    if (i < a.n) {
+      PlanItem x = a.items[i];
+      if (x.made) {
+        const int64_t needs = a.parents ? (x.len % a.BS ? 1 : 0) : pages_for(x.len, a.BS) - x.have;
+        none = needs > 0 && x.first + needs > found;
+        if (none) a.items[i].made = 0;
+        else if (a.parents && needs) a.items[i].dst = a.pages[x.first];
+      }
     }
-    block_scan(none, sum);
-    miss += sum;
+    miss += __syncthreads_count(none);
   }
   if (tid == 0) *a.short_out = static_cast<int32_t>(miss);
 }
@@ -182,18 +217,15 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanArgs
 __global__ void __launch_bounds__(256) pages_extend_kernel(const PlanArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t i = blockIdx.x;
-  const int64_t at = a.first[i];
-  if (at < 0) return;
-  const int64_t row = a.rows[i], len = a.lens[i];
-  const int64_t have = pages_for(a.seq_lens[row], a.BS), want = pages_for(len, a.BS);
-  __syncthreads();
-  for (int64_t b = have + threadIdx.x; b < want; b += blockDim.x) {
-    const int64_t page = a.pages[at + b - have];
-    a.table[row * a.s_bt + b] = static_cast<int32_t>(page);
+  const PlanItem x = a.items[blockIdx.x];
+  if (!x.made) return;
+  const int64_t want = pages_for(x.len, a.BS);
+  for (int64_t b = x.have + threadIdx.x; b < want; b += blockDim.x) {
+    const int64_t page = a.pages[x.first + b - x.have];
+    a.table[x.row * a.s_bt + b] = static_cast<int32_t>(page);
     a.refs[page] = 1;
   }
-  if (threadIdx.x == 0) a.seq_lens[row] = static_cast<int32_t>(len);
+  if (threadIdx.x == 0) a.seq_lens[x.row] = x.len;
 }
 
 // grid (1 + chunks of a page, items): part 0 makes the child's row, the others
@@ -201,30 +233,26 @@ __global__ void __launch_bounds__(256) pages_extend_kernel(const PlanArgs a) {
 __global__ void __launch_bounds__(256) pages_fork_kernel(const PlanArgs a, const PageTensors pt) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t i = blockIdx.y;
-  const int64_t at = a.first[i];
-  if (at < 0) return;
-  const int64_t par = a.parents[i], kid = a.rows[i];
-  const int64_t len = a.seq_lens[par];  // a parent is never a child of the same call: it holds tokens
-  const int64_t full = len / a.BS;
-  const bool part = len % a.BS != 0;
-  const int64_t page = part ? a.pages[at] : -1;
+  const PlanItem x = a.items[blockIdx.y];
+  if (!x.made) return;
   if (blockIdx.x > 0) {
-    const int64_t src = part ? a.table[par * a.s_bt + full] : -1;
-    if (src >= 0 && src < a.P) copy_chunk(pt, blockIdx.x - 1, src, page);
+    if (x.dst >= 0 && x.src >= 0 && x.src < a.P) copy_chunk(pt, blockIdx.x - 1, x.src, x.dst);
     return;
   }
+  const int64_t full = x.len / a.BS;
+  const int32_t* from = a.table + x.parent * a.s_bt;  // (a parent is never a child of the same call: it holds tokens)
+  int32_t* to = a.table + x.row * a.s_bt;
   for (int64_t b = threadIdx.x; b < full; b += blockDim.x) {
-    const int64_t p = a.table[par * a.s_bt + b];
-    a.table[kid * a.s_bt + b] = static_cast<int32_t>(p);
+    const int32_t p = from[b];
+    to[b] = p;
     if (p >= 0 && p < a.P) atomicAdd(&a.refs[p], 1);
   }
   if (threadIdx.x == 0) {
-    if (part) {
-      a.table[kid * a.s_bt + full] = static_cast<int32_t>(page);
-      a.refs[page] = 1;
+    if (x.dst >= 0) {
+      to[full] = x.dst;
+      a.refs[x.dst] = 1;
     }
-    a.seq_lens[kid] = static_cast<int32_t>(len);
+    a.seq_lens[x.row] = x.len;
   }
 }
 
@@ -246,22 +274,28 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  int64_t mine = 0, live;
-  for (int64_t p = tid; p < a.P; p += kPlanThreads) mine += a.refs[p] > 0;
+  // a thread's pages are neighbours, so two prefix sums do for any number of pages
+  const int64_t per = (a.P + kPlanThreads - 1) / kPlanThreads, lo = min(tid * per, a.P), hi = min(lo + per, a.P);
+  int64_t mine = 0, live, sum;
+  for (int64_t p = lo; p < hi; ++p) mine += a.refs[p] > 0;
   block_scan(mine, live);
-  int64_t ns = 0, nd = 0;
-  for (int64_t p0 = 0; p0 < a.P; p0 += kPlanThreads) {
-    const int64_t p = p0 + tid;
-    const bool used = p < a.P && a.refs[p] > 0;
-    const bool s = used && p >= live, d = p < a.P && !used && p < live;
-    int64_t sum;
-    const int64_t at = block_scan(s ? 1 : (d ? (1ll << 32) : 0), sum);  // both counts in one scan
-    if (s) a.src[ns + (at & 0xffffffff)] = static_cast<int32_t>(p);
-    if (d) a.dst[nd + (at >> 32)] = static_cast<int32_t>(p);
-    if (p < a.P) a.to[p] = static_cast<int32_t>(p);
-    ns += sum & 0xffffffff;
-    nd += sum >> 32;
+  // pages in use at or past `live` (low half), free ones below it (high half)
+  const int64_t used_past = hi <= live ? 0 : lo >= live ? mine : -1, below = min(max(live - lo, static_cast<int64_t>(0)), hi - lo);
+  int64_t ns = used_past, nd;
+  if (ns < 0) {
+    ns = 0;
+    for (int64_t p = live; p < hi; ++p) ns += a.refs[p] > 0;
   }
+  nd = below - (mine - ns);
+  int64_t at = block_scan(ns | (nd << 32), sum);
+  int32_t *src = a.src + (at & 0xffffffff), *dst = a.dst + (at >> 32);
+  for (int64_t p = lo; p < hi; ++p) {
+    const bool used = a.refs[p] > 0;
+    if (used && p >= live) *src++ = static_cast<int32_t>(p);
+    if (!used && p < live) *dst++ = static_cast<int32_t>(p);
+    a.to[p] = static_cast<int32_t>(p);
+  }
+  ns = sum & 0xffffffff;
   __syncthreads();
   if (a.out_refs != a.refs) {
     for (int64_t p = tid; p < a.P; p += kPlanThreads) a.out_refs[p] = a.refs[p];
@@ -327,15 +361,15 @@ static int check_pool(const int32_t* table, int64_t s_bt, int64_t R, int64_t W, 
 }
 
 extern "C" size_t srswa_pages_workspace_size(int64_t n, int64_t R, int64_t P) {
-  return static_cast<size_t>((n > 0 ? n : 0) + (R > 0 ? R : 0) + (P > 0 ? P : 0)) * 4;
+  return static_cast<size_t>(n > 0 ? n : 0) * sizeof(PlanItem) + static_cast<size_t>((R > 0 ? R : 0) + (P > 0 ? P : 0)) * 4;
 }
 
 static int make_plan(PlanArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   SRSWA_CHECK_ARG(workspace && workspace_bytes >= srswa_pages_workspace_size(a.n, a.R, a.P), SRSWA_EWORKSPACE);
-  SRSWA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 3) == 0, SRSWA_EALIGN);
-  a.claim = static_cast<int32_t*>(workspace);
-  a.first = a.claim + a.R;
-  a.pages = a.first + a.n;
+  SRSWA_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, SRSWA_EALIGN);
+  a.items = static_cast<PlanItem*>(workspace);
+  a.claim = reinterpret_cast<int32_t*>(a.items + a.n);
+  a.pages = a.claim + a.R;
   return launch_pdl(pages_plan_kernel, dim3(1), kPlanThreads, 0, st, a);
 }
 
