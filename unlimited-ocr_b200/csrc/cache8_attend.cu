@@ -9,7 +9,8 @@
 //   * codes widen to f16 exactly; q is scaled by a power of two so that it is
 //     exact in f16 too (bf16 elements under 2^-28 of the row's largest lose
 //     bits that fp32 sums would not show);
-//   * softmax weights are rounded to f16 (they are <= 1: 2^-11 relative).
+//   * softmax weights, times 2^15, are rounded to f16 (2^-11 relative down to
+//     2^-29 of a row's largest, where f16 runs out of exponents).
 // Both scales are applied in fp32, outside the MMAs.
 //
 // What bounds it: bytes.  A key costs 2 D bytes and 4 D flops per query head,
@@ -25,8 +26,10 @@
 // warp, so uneven lengths leave no tail and warps never wait for one another;
 // an item cut in several parts leaves fp32 partials that cache8_merge_kernel
 // joins in order.  Where the items are few and short the join would cost more
-// than the balance gives: there the four warps of a CTA share an item.  A warp streams its units through a private cp.async ring;
-// page ids, scales and biases are prefetched a block of 32 slots ahead.
+// than the balance gives: there the warps of a CTA share an item, and where they
+// are many and short each warp has an item of its own (rows_plan).  A warp
+// streams its units through a private cp.async ring; page ids, scales and biases
+// are prefetched a block of 32 slots ahead.
 
 #include <cmath>
 #include <type_traits>
@@ -36,15 +39,9 @@
 
 namespace srswa {
 
-constexpr int kRowsThreads = 128;
-constexpr int kRowsWarps = kRowsThreads / 32;
+constexpr float kRowsShift = 15.f;  // weights, their sums and the outputs are kept times 2^15
 constexpr int kRowsRing = 16384;  // shared memory of a warp's ring at D = 128 (half of it at 64)
-constexpr int kRowsCtasPerSm = 3;
 constexpr int kRowsCtaWarps = 6;  // of a CTA whose warps share an item, where there is room for two on each SM
-#ifndef PREFER_CH
-#define PREFER_CH 2
-#endif
-constexpr int kPreferCh = PREFER_CH;
 constexpr int kMaxSelected = 512;
 constexpr int kCols = 8;  // queries that share a pass over the keys (columns of the MMA)
 
@@ -394,10 +391,11 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
         m0 = n0m;
         m1 = n1m;
       }
+      const float e0 = u0 - kRowsShift, e1 = u1 - kRowsShift;
       uint32_t pb[CH][2];
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const float p0 = ex2(x[c][0] - u0), p1 = ex2(x[c][1] - u1), p2 = ex2(x[c][2] - u0), p3 = ex2(x[c][3] - u1);
+        const float p0 = ex2(x[c][0] - e0), p1 = ex2(x[c][1] - e1), p2 = ex2(x[c][2] - e0), p3 = ex2(x[c][3] - e1);
         l0 += p0 + p2;
         l1 += p1 + p3;
         pb[c][0] = transpose8x8(pack_half2(p0, p1));
@@ -419,7 +417,7 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
         // rows of the group see different keys: each takes the unit with the
         // keys that it does not see zeroed (their codes may be NaN), or not at
         // all (the page's scale may be)
-        for (int r = 0; r < share; ++r) {
+        for (int r = grp * kCols / G; r <= min((grp * kCols + kCols - 1) / G, share - 1); ++r) {
           uint32_t wr[CH][4][D / 32];
 #pragma unroll
           for (int c = 0; c < CH; ++c)
@@ -473,7 +471,7 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
         for (int e = 0; e < 2 * KS; ++e) x[e] = any ? x[e] / l : 0.f;
 #pragma unroll
         for (int e = 0; e < 2 * KS; e += 8) store8(a.out, n * a.s_on + h * a.s_oh + g * 2 * KS + e, a.out_dtype, x + e);
-        if (g == 0 && a.lse) a.lse[n * a.H + h] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (g == 0 && a.lse) a.lse[n * a.H + h] = any ? (m - kRowsShift + log2f(l)) * kLn2 : -INFINITY;
       } else {
         float4* p = reinterpret_cast<float4*>(po + col * D + g * 2 * KS);
 #pragma unroll
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
   const int64_t groups = a.N / share;
   int64_t req, pos, stop, rg, off;
   Span s;
-  if (a.split == kSplitCta) {  // a quarter of the CTA's item
+  if (a.split == kSplitCta) {  // a part of the CTA's item
     rg = blockIdx.x / per_group;
     s = group_span<CH>(a, rg, req);
     pos = s.units * warp / NW;
@@ -576,7 +574,7 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
   }
   if (a.split == kSplitEqual) {
     if (lane == 0) reinterpret_cast<int4*>(a.part_meta)[me] = make_int4(head_rg, head_item, tail_rg, tail_item);
-  } else if (a.split == kSplitCta) {  // join the four parts
+  } else if (a.split == kSplitCta) {  // join the warps' parts
     __syncthreads();
     const int64_t it = blockIdx.x % per_group, hk = it / a.ngrp, row0 = blockIdx.x / per_group * share;
     const int first = static_cast<int>(it % a.ngrp) * kCols, ncol = min(share * G - first, kCols);
@@ -596,7 +594,7 @@ __global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cac
       const bool any = L > 0.f || L != L;
       const int64_t n = row0 + gc / G, h = hk * G + gc % G;
       store_elem(a.out, n * a.s_on + h * a.s_oh + d, a.out_dtype, any ? x / L : 0.f);
-      if (d == 0 && a.lse) a.lse[n * a.H + h] = any ? (M + log2f(L)) * kLn2 : -INFINITY;
+      if (d == 0 && a.lse) a.lse[n * a.H + h] = any ? (M - kRowsShift + log2f(L)) * kLn2 : -INFINITY;
     }
   }
 }
@@ -671,10 +669,10 @@ __global__ void __launch_bounds__(128) cache8_merge_kernel(const Attend8Args a, 
     const float x = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
     store_elem(a.out, n * a.s_on + h * a.s_oh + tid, a.out_dtype, any ? x / L : 0.f);
   }
-  if (tid == 0 && a.lse) a.lse[n * a.H + h] = any ? (M + log2f(L)) * kLn2 : -INFINITY;
+  if (tid == 0 && a.lse) a.lse[n * a.H + h] = any ? (M - kRowsShift + log2f(L)) * kLn2 : -INFINITY;
 }
 
-static int sm_count() {
+int sm_count() {
   static int sms[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
@@ -694,7 +692,9 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   const int64_t groups = d.N / p.share;
   p.items = groups * d.Hkv * p.ngrp;
   // the most units an item can have
-  p.ch = d.block_size % 32 == 0 ? kPreferCh : 1;
+  // units of 32 keys where a page holds whole ones (16: 2 to 14 % slower on the
+  // same pages from 512 keys up, 196 against 215 us for 512 requests of 2048)
+  p.ch = d.block_size % 32 == 0 ? 2 : 1;
   const int64_t upp = d.block_size / (16 * p.ch);
   int64_t blocks = d.W;
   if (d.window >= 0) {
@@ -707,22 +707,39 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   int64_t parts = p.items;
   p.warps = kRowsWarps;
   p.split = kSplitNone;
+  p.units = p.items * most;
+  const int64_t wave = slots / kRowsWarps;  // CTAs of four warps at a time
   if (d.nsplit > 0) {
     if (d.nsplit > 1) p.split = kSplitEqual;
     parts = d.nsplit * p.items;
-  } else if (p.items <= slots / kRowsWarps && most <= 16 * kRowsWarps) {
-    // one wave of CTAs, at most 16 units a warp (measured: the table of
-    // cache8_rows_kernel)
-    p.split = kSplitCta;
-    if (p.items <= slots / kRowsCtaWarps) p.warps = kRowsCtaWarps;
-    parts = p.items * p.warps;
-  } else if (most <= 2 || groups > 2048 || p.items > 16 * slots || (p.items >= slots && most <= 16)) {
-    // items that a warp is through with at once, or so many that their uneven
-    // ends do not show: one warp each, no join
   } else {
-    p.split = kSplitEqual;
-    const int64_t enough = (p.items * most + 1) / 2;  // two units each at least
-    parts = enough < slots ? enough : slots;
+    // The three ways, in us for n requests of 16 / 4 heads of 128 and L keys (4 n
+    // items of L / 32 units; one warp each, a CTA each, equal parts):
+    //     n    L=128           256             512             1024            2048
+    //     1    10.9  7.2 12.3  15.3  8.3 13.0  24.1 10.4 12.7  41.6 14.4 13.0  76.2 22.5 14.2
+    //    16    11.3  7.8 12.4  15.7  9.5 13.2  24.6 11.7 13.6  42.2 17.0 15.9  77.1 24.9 23.7
+    //    64    12.2  8.6 14.8  17.2 10.3 15.8  26.0 12.9 22.7  43.8 18.8 27.5  80.9 32.7 42.1
+    //   128    14.2 15.5 16.3  21.3 18.1 23.0  35.3 24.2 27.7  64.9 45.0 42.6 120.1 73.4 64.2
+    //   256    15.7 23.1 25.9  24.0 28.6 30.7  42.4 44.7 45.4  73.2 70.2 66.9 134.0 115.5 109.0
+    //  1024    45.8 83.5 67.9  71.6 103  89.1  116   141  125   205   228  202   379   389  362
+    // A join of parts costs about 6 us; a warp or a CTA per item leaves the long
+    // items' ends alone on the GPU, so neither takes items of many units.
+    const bool many = p.items > wave && most * slots <= 20 * p.items;  // one warp each while the others have items too
+    const int64_t cap = 12 * p.items / slots > 16 ? 12 * p.items / slots : 16;
+    const int64_t warps = p.items * kRowsCtaWarps <= slots ? kRowsCtaWarps : kRowsWarps;
+    if (groups > 2048 || (many && most <= cap)) {
+      // (over 2048 groups each warp's search for its equal part costs more than
+      // the balance gives: 2500 requests of 1024 keys 439, equal parts 454)
+    } else if (2 * p.items <= 3 * wave && most <= (p.items <= wave ? 64 : 16) &&
+               5 * most * slots <= warps * (20 * slots + 6 * p.units)) {
+      p.split = kSplitCta;  // a warp's units, most / warps, at most 4 + 1.2 times an equal part
+      p.warps = static_cast<int>(warps);
+      parts = p.items * p.warps;
+    } else {
+      p.split = kSplitEqual;
+      const int64_t enough = (p.units + 1) / 2;  // two units each at least
+      parts = enough < slots ? enough : slots;
+    }
   }
   p.ctas = (parts + p.warps - 1) / p.warps;
   if (p.split == kSplitEqual) {

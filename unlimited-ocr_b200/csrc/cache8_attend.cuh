@@ -5,7 +5,7 @@
 
 namespace srswa {
 
-// One warp per item; the four warps of a CTA per item; equal parts of all units per warp.
+// One warp per item; the warps of a CTA per item; equal parts of all units per warp.
 enum { kSplitNone = 0, kSplitCta = 1, kSplitEqual = 2 };
 
 struct Attend8Args {
@@ -71,11 +71,15 @@ __device__ __forceinline__ float ex2(float x) {
 }
 struct RowsPlan {
   int64_t share, ngrp, items, ctas, o_floats;
+  int64_t units;  // of all items, at most
   size_t bytes;  // workspace
   int split;
   int ch;     // 16-key chunks of a unit
   int warps;  // of a CTA
 };
+constexpr int kRowsWarps = 4;  // of a CTA of the row kernel (plan.warps may be more), and CTAs an SM holds
+constexpr int kRowsCtasPerSm = 3;
+int sm_count();
 RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen);
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st);
 

@@ -33,6 +33,7 @@
 // that some row sees only in part have NaN value codes replaced by 0 and marked:
 // a row that does see one turns to NaN.
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -127,6 +128,12 @@ struct PrTile {
   __device__ __forceinline__ bool whole(int s, int i) const {
     const int k0 = key(i), k1 = k0 + kPrKeys - 1;
     return k1 <= first(s) && k1 < key_end(i) && (k0 > last(s) - win || k1 < sinks);
+  }
+
+  // some row that takes step i does not see all of it: its NaN value codes are
+  // taken out of the value tile and marked
+  __device__ __forceinline__ bool marked(int i) const {
+    return (needs(0, i) && !whole(0, i)) || (needs(1, i) && !whole(1, i));
   }
 
   __device__ __forceinline__ bool set(const Attend8Args& a, int64_t tile, int G) {
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
     float m = -INFINITY, l = 0.f, lref = -126.f;  // lref: log2 of vref
     bool poison = false, ok = true;
     int cnt = 0;
-    uint32_t seen[4];   // keys that this row saw of a step seen in part, until its
+    uint32_t seen[4];   // keys that this row saw of a marked step, until its
     int seen_at = -1;   // NaN words are known (the value tile is ready by the next S)
     auto check_nan = [&]() {
       if (seen_at < 0) return;
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       tmem_wait_st();
       tc_fence_before();
       pr_arrive(&p_full[s]);
-      if (KVT != SRSWA_I8 && !whole) {
+      if (KVT != SRSWA_I8 && T.marked(i)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) seen[c] = sees(c);
         seen_at = i & 15;
@@ -564,8 +571,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         load_codes(a.k, off, kx);
       }
       if (KVT != SRSWA_I8) {
-        const bool whole = (!T.needs(0, i) || T.whole(0, i)) && (!T.needs(1, i) || T.whole(1, i));
-        if (!whole) {
+        if (T.marked(i)) {
 #pragma unroll
           for (int j = 0; j < NP; ++j) {
             uint32_t* w = &vx[j].x;
@@ -668,18 +674,31 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
   }
 }
 
-// Rows without a selection, enough of them per request for a tile to be worth
-// its 128 keys a step: a 256-row pair of tiles costs about as much as 16 rows of
-// the row kernel over the same keys.
+// CTAs of a KV head: pairs of tiles of 128 / G tokens each (of ragged prompts,
+// the most there can be).
+static int64_t tile_pairs(int64_t N, int64_t R, int64_t rows_per_req, int64_t G, bool varlen) {
+  const int64_t pair = 2 * (128 / G);
+  return varlen ? N / pair + R : R * ((rows_per_req + pair - 1) / pair);
+}
+
+// Rows without a selection, where the tiles take less time than the row kernel
+// would, by what both cost (microseconds): the tiles 11 and 2.7 a step of 128
+// keys, for each wave of CTAs; the rows 10 and 2.4 per unit of 32 keys that a
+// warp has.
 bool prompt_applies(const srswa_cache8_desc& d, bool varlen) {
   const int64_t G = d.H / d.Hkv;
   if (d.K > 0 || G > 128 || d.nsplit > 0) return false;
-  return varlen ? d.N >= 16 * d.R : d.rows_per_req >= 16;
+  const double sms = sm_count();
+  const double waves = std::ceil(static_cast<double>(tile_pairs(d.N, d.R, d.rows_per_req, G, varlen)) * d.Hkv / sms);
+  double keys = static_cast<double>(d.W) * d.block_size;
+  if (d.window >= 0) keys = std::min(keys, static_cast<double>(d.window) + d.sinks + 2 * (128 / G));
+  const RowsPlan rows = rows_plan(d, varlen);
+  const double units = static_cast<double>(rows.units) * rows.ch / 2;
+  return waves * (11 + 2.7 * std::ceil(keys / kPrKeys)) < 10 + 2.4 * units / (kRowsCtasPerSm * kRowsWarps * sms);
 }
 
 int prompt_launch(const Attend8Args& a, int kv_dtype, int* status, cudaStream_t st) {
-  const int64_t tt = 128 / (a.H / a.Hkv);
-  const int64_t tiles = a.rows.cu ? a.N / (2 * tt) + a.rows.R : a.rows.R * ((a.rows.rps + 2 * tt - 1) / (2 * tt));
+  const int64_t tiles = tile_pairs(a.N, a.rows.R, a.rows.rps, a.H / a.Hkv, a.rows.cu != nullptr);
   if (tiles >= (1ll << 31)) return SRSWA_ETOOLARGE;
   SRSWA_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(int), st));
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.Hkv));
