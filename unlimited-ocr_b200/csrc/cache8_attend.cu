@@ -40,8 +40,16 @@
 namespace srswa {
 
 constexpr float kRowsShift = 15.f;  // weights, their sums and the outputs are kept times 2^15
-constexpr int kRowsRing = 16384;  // shared memory of a warp's ring at D = 128 (half of it at 64)
-constexpr int kRowsCtaWarps = 6;  // of a CTA whose warps share an item, where there is room for two on each SM
+// Warps of a CTA whose warps share an item: where an SM has one such CTA, and two
+// (of 128 features four warps with room for three units in flight take 18.0 us
+// where six with two take 19.0: 64 requests of 16 / 4 heads, 1024 keys; of 64
+// features six are faster, 14.5 and 15.3 us for 128 requests of 14 / 2 heads).
+constexpr int alone_warps(int D) { return D == 128 ? 8 : 12; }
+constexpr int pair_warps(int D) { return D == 128 ? 4 : 6; }
+// Shared memory of a warp's ring, D = 128: three units of 32 keys; 64: two (four
+// are no faster, and eight warps an SM with 24 KB each beat twelve with 16 KB
+// at D = 128: 134 and 139 us for the 750 MB of 16 requests of 37k to 62k keys).
+constexpr int ring_bytes(int D) { return D == 128 ? 24576 : 8192; }
 constexpr int kMaxSelected = 512;
 constexpr int kCols = 8;  // queries that share a pass over the keys (columns of the MMA)
 
@@ -111,10 +119,10 @@ __device__ __forceinline__ uint32_t v_off(int r, int c) {
 // page's chunks; two amortise the softmax bookkeeping and keep two independent
 // MMA chains going).
 template <int D, int KVT, int CH, bool MULTI, int NW>
-__global__ void __launch_bounds__(32 * NW, kRowsCtasPerSm * kRowsWarps / NW) cache8_rows_kernel(const Attend8Args a) {
+__global__ void __launch_bounds__(32 * NW, NW == alone_warps(D) ? 1 : 2) cache8_rows_kernel(const Attend8Args a) {
   constexpr int CB = 16 * D;           // bytes of a chunk of K (or V)
   constexpr int SB = 2 * CH * CB;      // bytes of a stage: K of its chunks, then V
-  constexpr int ST = kRowsRing * D / 128 / SB;  // stages of a warp's ring
+  constexpr int ST = ring_bytes(D) / SB;  // stages of a warp's ring
   constexpr int UK = 16 * CH;          // keys of a unit
   constexpr int KS = D / 16;           // MMA steps of a dot product, and feature tiles of the output
   constexpr int RPI = 512 / D;         // key rows per warp copy instruction
@@ -693,7 +701,7 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   p.items = groups * d.Hkv * p.ngrp;
   // the most units an item can have
   // units of 32 keys where a page holds whole ones (16: 2 to 14 % slower on the
-  // same pages from 512 keys up, 196 against 215 us for 512 requests of 2048)
+  // same pages from 512 keys up, as 215 for 196 us for 512 requests of 2048)
   p.ch = d.block_size % 32 == 0 ? 2 : 1;
   const int64_t upp = d.block_size / (16 * p.ch);
   int64_t blocks = d.W;
@@ -715,18 +723,21 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   } else {
     // The three ways, in us for n requests of 16 / 4 heads of 128 and L keys (4 n
     // items of L / 32 units; one warp each, a CTA each, equal parts):
-    //     n    L=128           256             512             1024            2048
-    //     1    10.9  7.2 12.3  15.3  8.3 13.0  24.1 10.4 12.7  41.6 14.4 13.0  76.2 22.5 14.2
-    //    16    11.3  7.8 12.4  15.7  9.5 13.2  24.6 11.7 13.6  42.2 17.0 15.9  77.1 24.9 23.7
-    //    64    12.2  8.6 14.8  17.2 10.3 15.8  26.0 12.9 22.7  43.8 18.8 27.5  80.9 32.7 42.1
-    //   128    14.2 15.5 16.3  21.3 18.1 23.0  35.3 24.2 27.7  64.9 45.0 42.6 120.1 73.4 64.2
-    //   256    15.7 23.1 25.9  24.0 28.6 30.7  42.4 44.7 45.4  73.2 70.2 66.9 134.0 115.5 109.0
-    //  1024    45.8 83.5 67.9  71.6 103  89.1  116   141  125   205   228  202   379   389  362
+    //     n   L=128               256                  512                  1024                 2048
+    //     1  10.6   7.9  12.8   14.5   7.6  12.9   22.2   8.8  12.8   37.7  11.8  12.9   68.4  17.4  13.8
+    //    16  10.9   7.1  11.8   14.9   7.6  12.7   22.7   9.2  13.1   38.3  12.2  14.9   69.4  17.7  19.2
+    //    64  11.4   8.0  14.2   16.1   9.5  14.8   23.9  12.3  20.2   41.8  17.8  24.4   81.8  31.3  38.0
+    //   128  12.1  14.5  15.3   17.2  17.3  20.8   27.9  23.0  25.0   50.7  38.0  38.4   91.6  59.0  59.4
+    //   256  12.6  26.8  23.7   18.2  32.5  29.4   31.9  50.2  41.9   53.2  71.8  63.0   95.6 108.2 101.3
+    //  1024  54.3 104.2  71.2   77.1 129.0  96.8  114.6 168.9 131.5  192.6 241.0 196.1  347.6 390.3 349.4
+    // (pages in L2 up to 128 MB).  Over 13 x 8 sizes of 16 / 4 and 10 / 10 heads the
+    // rules below take 1.5 % more than the best of the three.
     // A join of parts costs about 6 us; a warp or a CTA per item leaves the long
     // items' ends alone on the GPU, so neither takes items of many units.
     const bool many = p.items > wave && most * slots <= 20 * p.items;  // one warp each while the others have items too
     const int64_t cap = 12 * p.items / slots > 16 ? 12 * p.items / slots : 16;
-    const int64_t warps = p.items * kRowsCtaWarps <= slots ? kRowsCtaWarps : kRowsWarps;
+    const int64_t warps = p.items <= sm_count() ? alone_warps(static_cast<int>(d.D))
+                          : p.items <= 2 * sm_count() ? pair_warps(static_cast<int>(d.D)) : kRowsWarps;
     if (groups > 2048 || (many && most <= cap)) {
       // (over 2048 groups each warp's search for its equal part costs more than
       // the balance gives: 2500 requests of 1024 keys 439, equal parts 454)
@@ -754,7 +765,7 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
 template <int D, int KVT, int CH, bool MULTI, int NW>
 static int rows_start(const Attend8Args& a, unsigned ctas, cudaStream_t st) {
   auto kern = cache8_rows_kernel<D, KVT, CH, MULTI, NW>;
-  const int ring = NW * kRowsRing * D / 128;
+  const int ring = NW * ring_bytes(D);
   static bool allowed[64] = {};  // per device: the shared memory has been asked for
   int dev = 0;
   SRSWA_CUDA_TRY(cudaGetDevice(&dev));
@@ -778,8 +789,9 @@ int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace,
   auto by_warps = [&](auto d_, auto ch_, auto type_, auto multi_) -> int {
     constexpr int D = decltype(d_)::value, CH = decltype(ch_)::value, KVT = decltype(type_)::value;
     constexpr bool MULTI = decltype(multi_)::value;
-    return p.warps == kRowsWarps ? rows_start<D, KVT, CH, MULTI, kRowsWarps>(a, ctas, st)
-                                 : rows_start<D, KVT, CH, MULTI, kRowsCtaWarps>(a, ctas, st);
+    return p.warps == kRowsWarps      ? rows_start<D, KVT, CH, MULTI, kRowsWarps>(a, ctas, st)
+           : p.warps == pair_warps(D) ? rows_start<D, KVT, CH, MULTI, pair_warps(D)>(a, ctas, st)
+                                      : rows_start<D, KVT, CH, MULTI, alone_warps(D)>(a, ctas, st);
   };
   auto by_type = [&](auto d_, auto ch_) -> int {
     using I8 = std::integral_constant<int, SRSWA_I8>;

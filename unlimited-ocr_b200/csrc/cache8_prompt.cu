@@ -683,8 +683,10 @@ static int64_t tile_pairs(int64_t N, int64_t R, int64_t rows_per_req, int64_t G,
 
 // Rows without a selection, where the tiles take less time than the row kernel
 // would, by what both cost (microseconds): the tiles 11 and 2.7 a step of 128
-// keys, for each wave of CTAs; the rows 10 and 2.4 per unit of 32 keys that a
-// warp has.
+// keys, for each wave of CTAs; the rows 10 and 1.6 per unit of 32 keys that a
+// resident warp has.  (16 / 4 heads of 128, rows and tiles: 16 rows after 4096 keys
+// 33 and 98, 32 requests of them 196 and 105; 300 such ragged rows in 4 requests
+// 166 and 112.  Over 585 sizes the choice takes 2 % more than the better one.)
 bool prompt_applies(const srswa_cache8_desc& d, bool varlen) {
   const int64_t G = d.H / d.Hkv;
   if (d.K > 0 || G > 128 || d.nsplit > 0) return false;
@@ -694,7 +696,7 @@ bool prompt_applies(const srswa_cache8_desc& d, bool varlen) {
   if (d.window >= 0) keys = std::min(keys, static_cast<double>(d.window) + d.sinks + 2 * (128 / G));
   const RowsPlan rows = rows_plan(d, varlen);
   const double units = static_cast<double>(rows.units) * rows.ch / 2;
-  return waves * (11 + 2.7 * std::ceil(keys / kPrKeys)) < 10 + 2.4 * units / (kRowsCtasPerSm * kRowsWarps * sms);
+  return waves * (11 + 2.7 * std::ceil(keys / kPrKeys)) < 10 + 1.6 * units / (kRowsCtasPerSm * kRowsWarps * sms);
 }
 
 int prompt_launch(const Attend8Args& a, int kv_dtype, int* status, cudaStream_t st) {
