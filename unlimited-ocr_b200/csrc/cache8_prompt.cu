@@ -31,7 +31,8 @@
 // Codes that a row does not see must not reach it: masked scores are replaced
 // before use, weights of masked keys are 0, and because 0 * NaN is not, steps
 // that some row sees only in part have NaN value codes replaced by 0 and marked:
-// a row that does see one turns to NaN.
+// a row that does see one turns to NaN (by its mask, or with its whole tile where
+// only the pair's other tile sees the step in part).
 
 #include <algorithm>
 #include <cmath>
@@ -130,12 +131,6 @@ struct PrTile {
     return k1 <= first(s) && k1 < key_end(i) && (k0 > last(s) - win || k1 < sinks);
   }
 
-  // some row that takes step i does not see all of it: its NaN value codes are
-  // taken out of the value tile and marked
-  __device__ __forceinline__ bool marked(int i) const {
-    return (needs(0, i) && !whole(0, i)) || (needs(1, i) && !whole(1, i));
-  }
-
   __device__ __forceinline__ bool set(const Attend8Args& a, int64_t tile, int G) {
     tt = 128 / G;
     int64_t lo = 0, hi = a.rows.R, nth;
@@ -203,7 +198,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
   // code, zeroed 4 steps ahead
   __shared__ __align__(16) float g_ks[8][8], g_lv[8][8];
   __shared__ float g_top[8];
-  __shared__ uint32_t g_on[8], g_nan[16][4];
+  __shared__ uint32_t g_on[8], g_nan[16][4], g_poison[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -221,6 +216,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
     tmem_relinquish();
   }
   if (tid < 64) g_nan[tid >> 2][tid & 3] = 0;
+  if (tid < 2) g_poison[tid] = 0;
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 128);
@@ -306,7 +302,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
     float m = -INFINITY, l = 0.f, lref = -126.f;  // lref: log2 of vref
     bool poison = false, ok = true;
     int cnt = 0;
-    uint32_t seen[4];   // keys that this row saw of a marked step, until its
+    uint32_t seen[4];   // keys that this row saw of a step seen in part, until its
     int seen_at = -1;   // NaN words are known (the value tile is ready by the next S)
     auto check_nan = [&]() {
       if (seen_at < 0) return;
@@ -438,7 +434,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       tmem_wait_st();
       tc_fence_before();
       pr_arrive(&p_full[s]);
-      if (KVT != SRSWA_I8 && T.marked(i)) {
+      if (KVT != SRSWA_I8 && !whole) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) seen[c] = sees(c);
         seen_at = i & 15;
@@ -451,6 +447,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         tc_fence_after();
         check_nan();
         const bool any = l > 0.f || l != l;
+        poison = poison || g_poison[s];
         const float inv = poison ? NAN : any ? exp2f(lref) / l : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -571,7 +568,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         load_codes(a.k, off, kx);
       }
       if (KVT != SRSWA_I8) {
-        if (T.marked(i)) {
+        const bool all0 = T.needs(0, i) && T.whole(0, i), all1 = T.needs(1, i) && T.whole(1, i);
+        if ((T.needs(0, i) && !all0) || (T.needs(1, i) && !all1)) {
 #pragma unroll
           for (int j = 0; j < NP; ++j) {
             uint32_t* w = &vx[j].x;
@@ -583,7 +581,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
               w[e] &= ~(nan * 0xffu);
             }
             const int kk = j * RPP + kr;
-            if (any) atomicOr(&g_nan[i & 15][kk >> 5], 1u << (kk & 31));
+            if (any) {
+              atomicOr(&g_nan[i & 15][kk >> 5], 1u << (kk & 31));
+              if (all0) g_poison[0] = 1;  // every row of that tile sees it
+              if (all1) g_poison[1] = 1;
+            }
           }
         }
       }
