@@ -723,7 +723,8 @@ SRSWA_API int srswa_rope2d_decode(const int64_t* new_ids, int64_t s_ids, int64_t
  * (features contiguous, any order of page / position / head).  Pages are named
  * by block_table [R, W] int32; an id outside [0, P) names no page and its
  * tokens are never read or written.  No counterpart in the reference, whose
- * fp8 cache has no scales (attend_triton.py:545, 626).
+ * fp8 cache has no scales (attend_triton.py:545, 626).  Scales are finite and
+ * not negative; D is 64 or 128, block_size a multiple of 16, K at most 512.
  *
  * Rows (query rows of the attend, new tokens of the append) come in two forms:
  *   cu_rows == NULL: row n belongs to request n / rows_per_req, at position
@@ -744,7 +745,7 @@ typedef struct {
   int64_t s_scale;       /* row stride of k_scale / v_scale [P, Hkv] */
   int64_t s_bt;          /* row stride of block_table */
   int64_t s_ti_h, s_ti_n, s_b_h, s_b_n;
-  int64_t nsplit;        /* attend: parts a row's keys are split into (0: chosen) */
+  int64_t nsplit;        /* attend: parts a row's keys are split into (0: chosen, and the kernel with it) */
 } srswa_cache8_desc;
 
 /* Append: quantises new tokens k, v [N, Hkv, D] (f32 / bf16 / f16; q_dtype)
@@ -769,9 +770,11 @@ SRSWA_API int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, con
  * sm_scale * q . k + bias over them; out [N, H, D] (out_dtype: q's type or F32)
  * and lse_out [N, H] fp32 natural log (optional).  A row that sees nothing
  * gives 0 and -inf.  Codes of keys that a row does not see never reach its
- * result, whatever they hold.  workspace: srswa_cache8_attend_workspace_size
- * bytes, 16-byte aligned (0: none); after a call with more than one part per
- * row its content is scratch. */
+ * result, whatever they hold; NaN in those that it sees does.  workspace:
+ * srswa_cache8_attend_workspace_size bytes, 16-byte aligned (0: none).  Calls
+ * with many rows per request go to tensor-core tiles: their workspace is 16
+ * bytes, whose first 4 are the call's status word (srswa_workspace_status); of
+ * the others it is scratch. */
 SRSWA_API size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen);
 SRSWA_API int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, const void* k_cache,
                                   const void* v_cache, const float* k_scale, const float* v_scale,

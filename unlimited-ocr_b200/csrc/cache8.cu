@@ -100,7 +100,8 @@ __device__ __forceinline__ void regrow(uint8_t* tile, int64_t s_pos, int held, f
 // memory: the new elements of a page stay in registers between the maximum and
 // the rounding (pages of up to 8 passes of the CTA; longer ones are read twice,
 // the second time from L2), so each is read once and its code written once.
-// 38k tokens of 10 heads of 128, bf16 to e4m3: see the table of measurements.
+// 132 MB of bf16 and e4m3 (nine ragged prompts of up to 7001 tokens, 10 heads of
+// 128): 29 us, 71 % of the copy rate; with 5 / 8 / 10 CTAs an SM for six 33 / 35 / 39.
 template <int D, int KVT>
 __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const AppendArgs a) {
   constexpr int LPT = D / 8;                     // lanes per token, 8 elements each
@@ -247,8 +248,9 @@ __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const 
 }
 
 // One new token per request (decode): one warp per (request, head, K or V), a
-// lane holds D / 32 features.  Bound by the latency of its four dependent reads
-// (length, page, scale; the elements come beside them).
+// lane holds D / 32 features.  Bound by the latency of its dependent reads (length,
+// page, scale; the elements come beside them): 256 requests of 10 heads 4.6 us a
+// call, 12.2 with the kernel above.
 template <int D, int KVT>
 __global__ void __launch_bounds__(kAppendThreads) cache8_append_one_kernel(const AppendArgs a) {
   constexpr int E = D / 32;

@@ -27,6 +27,15 @@
 // read codes from the pages, widen them and write the swizzled K / V tiles
 // (double buffered, the next step's codes already in registers); 12 issues the
 // MMAs and owns TMEM.  TMEM, per tile: S (128 columns; W over its first 64) and O.
+// (The next S overwrites W behind the product that reads it: one thread issues
+// both, and its MMAs execute in order.)
+//
+// Measured: 8192 rows of 16 / 4 heads of 128 after 8192 tokens 1040 us, 790
+// TFLOP/s, 47 % of the measured bf16 rate.  A step takes 4700 cycles where its
+// MMAs take 2048: the softmax of a tile takes 3300 (its exp2 share the unit with
+// the other tile's), and the steps of the two tiles do not interleave fully.
+// Ragged prompts with a window of 512 and 64 sinks, 10 heads: 86 us, three waves
+// of CTAs that each spend about 9 us on their first codes and their output.
 //
 // Codes that a row does not see must not reach it: masked scores are replaced
 // before use, weights of masked keys are 0, and because 0 * NaN is not, steps

@@ -867,7 +867,9 @@ def cache8_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens=N
     layout, or None.  sm_scale: 1 / sqrt(D) by default.  Returns out [N, H, D]
     (q's type, or the given out's: q's or fp32), with lse=True also the fp32
     log-sum-exp [N, H]; a row that sees nothing gives 0 and -inf.  nsplit: the
-    parts the keys of a row are cut into (0: chosen)."""
+    parts the keys of a row are cut into (0: chosen).  workspace: optional
+    caller uint8 tensor; after a call that tensor-core tiles took its first 4
+    bytes are the status word (workspace_status)."""
     return L.bind().attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens, window,
                            sinks, topk_idx, bias, sm_scale, out, lse, nsplit, workspace)
 
