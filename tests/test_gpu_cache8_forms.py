@@ -175,3 +175,11 @@ def test_example_beams(cuda, code):
                         cache.v_scale.double().cpu().numpy(), table, np.repeat(np.arange(len(rows)), n), pos,
                         r["window"], r["sinks"], None, None, ex.D ** -0.5)
     assert (np.abs(r["after"].double().cpu().numpy() - o) <= 2.0 ** -8 * np.abs(o) + 2.0 ** -10 * a + 1e-7).all()
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("lens", [[1], [300], [7, 0, 64, 900]])
+def test_rows_see_nothing(cuda, rows, lens):
+    """No window, no sinks, no selection: zeros and -inf."""
+    o = run_rows(cuda, np.random.default_rng(48), lens, rows, 8, 2, 128, 64, "int8", "bf16", 0, 0, 0)
+    assert (o == 0).all()

@@ -620,8 +620,8 @@ template <int D>
 __global__ void __launch_bounds__(128) cache8_merge_kernel(const Attend8Args a, int parts) {
   constexpr int V = D / 32;  // features of a lane
   __shared__ float wt[128], red[4][D], top[4];
-  // (no early launch of what follows: beside these CTAs a next attend would not fit
-  // three to an SM, and its equal parts want to start together: 171 us for 130)
+  // (no early launch of what follows: beside these CTAs a next attend would not get
+  // all its CTAs at once, and its equal parts want to start together: 171 us for 130)
   pdl_wait();
   const int c = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int4* meta = reinterpret_cast<const int4*>(a.part_meta);
