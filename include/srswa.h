@@ -731,7 +731,9 @@ SRSWA_API int srswa_rope2d_decode(const int64_t* new_ids, int64_t s_ids, int64_t
  *     seq_lens[r] - rows_per_req + n % rows_per_req (the last rows of each
  *     request; N = R * rows_per_req);
  *   cu_rows [R + 1]: rows cu_rows[r] <= n < cu_rows[r + 1] belong to request r,
- *     at position prefix_lens[r] + n - cu_rows[r] (varlen; cu_rows[R] = N). */
+ *     at position prefix_lens[r] + n - cu_rows[r] (varlen, cu_rows ascending).
+ *     Rows before cu_rows[0] and from cu_rows[R] on belong to no request: the
+ *     append ignores them, the attend gives 0 and -inf. */
 typedef struct {
   int64_t N, R, H, Hkv, D, P, W, block_size;
   int64_t rows_per_req;

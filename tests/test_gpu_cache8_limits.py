@@ -1,0 +1,126 @@
+"""The scaled 8-bit cache at the limits of its contract: value scales of any
+spread, table entries past a request's end, queries and biases at the ends of
+their types, requests shorter than their rows, rows of no request.
+
+Tolerance of the attend, from the arithmetic, for rows and tiles alike: softmax
+weights are rounded to f16 (2^-11 of each product p v), the rest is fp32 (the
+same again allowed, 2^-11 of sum p |v|, as in test_gpu_cache8.py), the output is
+rounded to its type.  f16 ends at 2^-24: the weights are kept such that the
+row's largest product of a weight and a value scale is at 2^7 or more, so each
+key may be off by 2^-25 / 2^7 of that times its code: 2^-32 max(p s) sum |code|."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache8 as O8
+from srswa import _lib as L
+from srswa import cache8, ops
+from test_gpu_cache8 import CODE, U, make_cache
+from test_gpu_cache8_forms import tiles_take
+
+pytestmark = pytest.mark.gpu
+
+
+def dense(q, vals, sc, table, req, pos, window, sinks, sm):
+    """o, lse, sum p |v| and max(p s) sum |code| of every row, in 64 bits."""
+    N, H, D = q.shape
+    P, BS, Hkv, _ = vals.shape[1:]
+    G = H // Hkv
+    o, a, f = (np.zeros((N, H, D)) for _ in range(3))
+    lse = np.full((N, H), -np.inf)
+    for r in np.unique(req):
+        n = np.nonzero(req == r)[0]
+        S = min(max(int(pos[n].max()) + 1, 0), table.shape[1] * BS)
+        j = np.arange(S)
+        page = table[r, j // BS]
+        there = (page >= 0) & (page < P)
+        page = np.where(there, page, 0)
+        p = pos[n][:, None]
+        seen = there & (j <= p)
+        if window is not None:
+            seen &= (j > p - window) | (j < sinks)
+        with np.errstate(invalid="ignore"):
+            for h in range(Hkv):
+                k = np.where(there[:, None], vals[0, page, j % BS, h] * sc[0, page, h][:, None], 0.0)
+                s = np.where(there, sc[1, page, h], 0.0)
+                c = np.where(there[:, None], vals[1, page, j % BS, h], 0.0)
+                for g in range(h * G, h * G + G):
+                    z = np.where(seen, q[n, g] @ k.T * sm, -np.inf)
+                    m = z.max(1, keepdims=True, initial=-np.inf)
+                    e = np.where(seen, np.exp(z - np.where(np.isfinite(m), m, 0.0)), 0.0)
+                    t = e.sum(1, keepdims=True)
+                    e /= np.where(t > 0, t, 1.0)
+                    lse[n, g] = np.where(t[:, 0] > 0, m[:, 0] + np.log(np.where(t > 0, t, 1.0))[:, 0], -np.inf)
+                    o[n, g] = (e * s) @ c
+                    a[n, g] = (e * s) @ np.abs(c)
+                    f[n, g] = (e * s).max(1, keepdims=True, initial=0.0) * (seen @ np.abs(c))
+    return o, lse, a, f
+
+
+def close(out, lse, ref):
+    o, l, a, f = ref
+    got = out.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    tol = U[out.dtype] * np.abs(o) + 2.0 ** -10 * a + 2.0 ** -32 * f
+    assert (np.abs(got - o) <= tol).all(), np.nanmax(np.abs(got - o) / np.where(tol > 0, tol, 1e-300))
+    g = lse.double().cpu().numpy()
+    assert np.array_equal(np.isneginf(g), np.isneginf(l))
+    fin = np.isfinite(l)
+    assert np.abs(g[fin] - l[fin]).max(initial=0.0) <= 1e-4
+
+
+def place(dev, form, lens, rows):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    pos = np.concatenate([n - rows + np.arange(rows) for n in lens])
+    req = np.repeat(np.arange(len(lens)), rows)
+    if form == "ragged":
+        return pos, req, dict(cu_seqlens=i32([rows * i for i in range(len(lens) + 1)]), prefix_lens=i32([n - rows for n in lens]))
+    return pos, req, dict(seq_lens=i32(lens))
+
+
+@pytest.mark.parametrize("code,real,BS", [("e4m3", "bf16", 64), ("int8", "f32", 16)])
+@pytest.mark.parametrize("ahead,behind", [(5, 0), (200, 0), (0, 77), (517, 300)])
+def test_append_rows_of_no_request(cuda, code, real, BS, ahead, behind):
+    """cu_seqlens may begin behind row 0 and end before the last row."""
+    rng = np.random.default_rng(66)
+    start, count = [0, 70, 3, 0], [65, 1, 0, 130]
+    R, Hkv, D, W = len(start), 2, 128, -(-130 // BS) + 1
+    real = {"bf16": torch.bfloat16, "f32": torch.float32}[real]
+    bt = torch.from_numpy(rng.permutation(R * W).astype(np.int32).reshape(R, W)).to(cuda)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    x = torch.from_numpy(rng.standard_normal((2, ahead + sum(count) + behind, Hkv, D))).to(cuda).to(real)
+    cu = np.array([0, *np.cumsum(count)])
+    a, b = (cache8.Cache8(R * W, BS, Hkv, D, dtype=CODE[code], device=cuda) for _ in range(2))
+    a.append(*x, bt, cu_seqlens=i32(cu + ahead), prefix_lens=i32(start))
+    b.append(*x[:, ahead: ahead + sum(count)], bt, cu_seqlens=i32(cu), prefix_lens=i32(start))
+    for s, t in zip(a.tensors(), b.tensors()):
+        assert torch.equal(*(y if y.dtype == torch.float32 else y.view(torch.uint8) for y in (s, t)))
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 4)])
+@pytest.mark.parametrize("ahead,behind", [(5, 0), (700, 0), (0, 77), (517, 1300)])
+@pytest.mark.parametrize("new", [[300, 1, 0, 469], [3, 1, 0, 4]])
+def test_attend_rows_of_no_request(cuda, window, sinks, ahead, behind, new):
+    """Such rows give 0 and -inf, and the others what they give without them."""
+    rng = np.random.default_rng(67)
+    pre, H, Hkv, D, BS = [0, 70, 3, 131], 8, 2, 128, 64
+    lens = [p + n for p, n in zip(pre, new)]
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    n = sum(new)
+    if n > 100:
+        assert tiles_take(N=ahead + n + behind, R=4, H=H, Hkv=Hkv, D=D, W=table.shape[1], P=30, block_size=BS,
+                          window=window or -1, sinks=sinks)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.from_numpy(rng.standard_normal((ahead + n + behind, H, D))).to(cuda).to(torch.bfloat16)
+    cu = np.array([0, *np.cumsum(new)])
+    out = torch.full(q.shape, math.nan, device=cuda, dtype=torch.float32)
+    o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), cu_seqlens=i32(cu + ahead),
+                               prefix_lens=i32(pre), window=window, sinks=sinks, lse=True, out=out)
+    mine = slice(ahead, ahead + n)
+    for part in (slice(0, ahead), slice(ahead + n, None)):
+        assert (o[part] == 0).all() and torch.isneginf(lse[part]).all()
+    pos, req = np.concatenate([a + np.arange(m) for a, m in zip(pre, new)]), np.repeat(np.arange(4), new)
+    close(o[mine], lse[mine], dense(q[mine].double().cpu().numpy(), vals, sc, table, req, pos, window, sinks, D ** -0.5))

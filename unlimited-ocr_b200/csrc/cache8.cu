@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const 
       before += here;
       if (here < kAppendThreads) break;
     }
+    if (before == 0) return;  // rows ahead of the first request's
     req = before - 1;
     row0 = a.rows.cu[req];
     nth = i - (row0 / a.BS + 2 * req);

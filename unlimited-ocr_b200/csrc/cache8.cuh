@@ -25,7 +25,8 @@ __device__ __forceinline__ void row_place(const RowMap& m, int64_t n, int64_t& r
       else hi = mid;
     }
     req = lo;
-    pos = static_cast<int64_t>(m.prefix[lo]) + n - m.cu[lo];
+    // a row of no request is ahead of every key
+    pos = n >= m.cu[lo] && n < m.cu[lo + 1] ? static_cast<int64_t>(m.prefix[lo]) + n - m.cu[lo] : -1;
   } else {
     req = n / m.rps;
     pos = static_cast<int64_t>(m.seq_lens[req]) - m.rps + n % m.rps;

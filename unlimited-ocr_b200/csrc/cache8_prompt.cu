@@ -154,6 +154,7 @@ struct PrTile {
       n = a.rows.cu[req + 1] - static_cast<int>(row0);
       p0 = a.rows.prefix[req];
       nth = tile - (row0 / (2 * tt) + req);
+      if (nth < 0) return false;  // ahead of the first request's rows
     } else {
       const int64_t per = (a.rows.rps + 2 * tt - 1) / (2 * tt);
       req = tile / per;
@@ -215,6 +216,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
   const int64_t hk = blockIdx.y;
   pdl_launch_dependents();
   pdl_wait();
+  if (a.rows.cu && blockIdx.x == 0) {  // rows of no request, as in a batch padded to a fixed size
+    const int64_t first = min(max(static_cast<int64_t>(a.rows.cu[0]), static_cast<int64_t>(0)), a.N);
+    const int64_t past = min(max(static_cast<int64_t>(a.rows.cu[a.rows.R]), first), a.N);
+    const float zero[8] = {};
+    for (int64_t i = tid; i < (first + a.N - past) * G * (D / 8); i += kPrThreads) {
+      const int64_t nth = i / (G * (D / 8)), row = nth < first ? nth : past + nth - first;
+      const int64_t h = hk * G + i / (D / 8) % G;
+      store8(a.out, row * a.s_on + h * a.s_oh + i % (D / 8) * 8, a.out_dtype, zero);
+      if (i % (D / 8) == 0 && a.lse) a.lse[row * a.H + h] = -INFINITY;
+    }
+  }
   PrTile T;
   // the last tiles of a prompt have the most keys: they go first
   if (!T.set(a, gridDim.x - 1 - blockIdx.x, G)) return;

@@ -849,7 +849,8 @@ def cache8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_len
     (float8_e4m3fn or int8; any strides with D contiguous), scales [P, Hkv]
     fp32.  Either the last N / R tokens of each request (seq_lens [R] int32
     counts them already), or varlen rows: request r's tokens are rows
-    cu_seqlens[r] .. cu_seqlens[r + 1] - 1, after prefix_lens[r] earlier ones.
+    cu_seqlens[r] .. cu_seqlens[r + 1] - 1, after prefix_lens[r] earlier ones
+    (rows of no request, before the first or behind the last, are ignored).
     Scales are powers of two; a page's scale grows when new tokens need it,
     and its earlier codes are rounded to the new scale (srswa_cache8_append)."""
     L.bind().append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, prefix_lens)
