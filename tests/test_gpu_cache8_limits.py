@@ -124,3 +124,33 @@ def test_attend_rows_of_no_request(cuda, window, sinks, ahead, behind, new):
         assert (o[part] == 0).all() and torch.isneginf(lse[part]).all()
     pos, req = np.concatenate([a + np.arange(m) for a, m in zip(pre, new)]), np.repeat(np.arange(4), new)
     close(o[mine], lse[mine], dense(q[mine].double().cpu().numpy(), vals, sc, table, req, pos, window, sinks, D ** -0.5))
+
+
+@pytest.mark.parametrize("form,rows", [("rows", 270), ("ragged", 270), ("rows", 1), ("rows", 5), ("ragged", 3)])
+@pytest.mark.parametrize("scale", [1e30, math.inf, math.nan])
+@pytest.mark.parametrize("window", [None, 100])
+def test_table_entries_past_the_end(cuda, form, rows, scale, window):
+    """Pages that the table names past a request's tokens (room reserved, or left
+    over from another request) do not reach its rows."""
+    rng = np.random.default_rng(62)
+    # 270 rows of 4 heads a KV head end in the first tile of their last pair, a few keys before a page's end
+    lens, H, Hkv, D, BS = [701, 318], 8, 2, 128, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    unused = np.setdiff1d(np.arange(len(ks)), table[table >= 0])
+    assert len(unused) >= 3
+    wide = np.full((2, table.shape[1] + 1), -1, np.int32)
+    wide[:, : table.shape[1]] = table
+    full = wide.copy()
+    for r in range(2):
+        full[r, -(-lens[r] // BS):] = unused[np.arange(full.shape[1] - -(-lens[r] // BS)) % len(unused)]
+    for x in (ks, vs):
+        x[torch.from_numpy(unused).to(cuda)] = scale
+    pos, req, at = place(cuda, form, lens, rows)
+    if rows > 64:
+        assert tiles_take(N=2 * rows, R=2, H=H, Hkv=Hkv, D=D, W=12, P=20, block_size=BS, window=window or -1,
+                          **({} if form == "ragged" else {"rows_per_req": rows}))
+    q = torch.from_numpy(rng.standard_normal((2 * rows, H, D))).to(cuda).to(torch.bfloat16)
+    run = lambda t: ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(t).to(cuda), window=window, lse=True, **at)  # noqa: E731
+    a, b = run(wide), run(full)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    close(*b, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, window, 0, D ** -0.5))

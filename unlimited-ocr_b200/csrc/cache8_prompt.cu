@@ -169,7 +169,7 @@ struct PrTile {
     constexpr int big = 0x7ffffe00;
     win = a.window < 0 ? big : static_cast<int>(min(a.window, static_cast<int64_t>(big)));
     sinks = static_cast<int>(min(a.sinks, static_cast<int64_t>(big)));
-    const int pl = max(last(0), last(1));
+    const int pl = p0 + min(tok0 + 2 * tt, n) - 1;  // the pair's last row (its second tile may be empty)
     end = static_cast<int>(max(min(static_cast<int64_t>(pl) + 1, min(a.W * a.BS, static_cast<int64_t>(big))),
                                static_cast<int64_t>(0)));
     const int ls = max(first(0) - win + 1, 0);
