@@ -7,7 +7,10 @@ weights are rounded to f16 (2^-11 of each product p v), the rest is fp32 (the
 same again allowed, 2^-11 of sum p |v|, as in test_gpu_cache8.py), the output is
 rounded to its type.  f16 ends at 2^-24: the weights are kept such that the
 row's largest product of a weight and a value scale is at 2^7 or more, so each
-key may be off by 2^-25 / 2^7 of that times its code: 2^-32 max(p s) sum |code|."""
+key may be off by 2^-25 / 2^7 of that times its code: 2^-32 max(p s) sum |code|.
+What lies under fp32's smallest normal, 2^-126, may be lost.  Scores are fp32 sums
+of exact products, so lse may be off by (D + 2) 2^-24 of the largest sum |q k|
+(1e-4 for the normal queries of test_gpu_cache8.py)."""
 
 import math
 
@@ -25,12 +28,13 @@ pytestmark = pytest.mark.gpu
 
 
 def dense(q, vals, sc, table, req, pos, window, sinks, sm):
-    """o, lse, sum p |v| and max(p s) sum |code| of every row, in 64 bits."""
+    """o, lse, sum p |v|, max(p s) sum |code| and the largest sum |q k| of every
+    row, in 64 bits."""
     N, H, D = q.shape
     P, BS, Hkv, _ = vals.shape[1:]
     G = H // Hkv
     o, a, f = (np.zeros((N, H, D)) for _ in range(3))
-    lse = np.full((N, H), -np.inf)
+    lse, y = np.full((N, H), -np.inf), np.zeros((N, H))
     for r in np.unique(req):
         n = np.nonzero(req == r)[0]
         S = min(max(int(pos[n].max()) + 1, 0), table.shape[1] * BS)
@@ -57,19 +61,20 @@ def dense(q, vals, sc, table, req, pos, window, sinks, sm):
                     o[n, g] = (e * s) @ c
                     a[n, g] = (e * s) @ np.abs(c)
                     f[n, g] = (e * s).max(1, keepdims=True, initial=0.0) * (seen @ np.abs(c))
-    return o, lse, a, f
+                    y[n, g] = np.where(seen, np.abs(q[n, g]) @ np.abs(k.T), 0.0).max(1, initial=0.0) * abs(sm)
+    return o, lse, a, f, y
 
 
 def close(out, lse, ref):
-    o, l, a, f = ref
+    o, l, a, f, y = ref
     got = out.double().cpu().numpy()
     assert np.isfinite(got).all()
-    tol = U[out.dtype] * np.abs(o) + 2.0 ** -10 * a + 2.0 ** -32 * f
+    tol = U[out.dtype] * np.abs(o) + 2.0 ** -10 * a + 2.0 ** -32 * f + 2.0 ** -126
     assert (np.abs(got - o) <= tol).all(), np.nanmax(np.abs(got - o) / np.where(tol > 0, tol, 1e-300))
     g = lse.double().cpu().numpy()
     assert np.array_equal(np.isneginf(g), np.isneginf(l))
     fin = np.isfinite(l)
-    assert np.abs(g[fin] - l[fin]).max(initial=0.0) <= 1e-4
+    assert (np.abs(g[fin] - l[fin]) <= np.maximum(1e-4, (o.shape[2] + 2) * 2.0 ** -24 * y[fin])).all()
 
 
 def place(dev, form, lens, rows):
@@ -154,3 +159,32 @@ def test_table_entries_past_the_end(cuda, form, rows, scale, window):
     a, b = run(wide), run(full)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     close(*b, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, window, 0, D ** -0.5))
+
+
+SPREADS = {"neighbours": lambda b: 30 * (b % 2) - 15, "steps": lambda b: 70 * (b // 2 % 2) - 50, "up": lambda b: 5 * b - 40,
+           "down": lambda b: 10 - 5 * b, "thirds": lambda b: [-110, 0, 90][b % 3], "none": lambda b: [0, None][b % 2],
+           "all none": lambda b: None}
+
+
+@pytest.mark.parametrize("spread", list(SPREADS))
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3), (200, 0)])
+@pytest.mark.parametrize("rows,form,code,D", [(300, "rows", "e4m3", 128), (270, "ragged", "int8", 64)])
+def test_value_scales_of_any_spread(cuda, spread, window, sinks, rows, form, code, D):
+    """Value scales up to 2^200 apart, or 0, from page to page: every row as good
+    as its own keys allow, whatever its neighbours see."""
+    rng = np.random.default_rng(60)
+    lens, H, Hkv, BS = [700, 350], 8, 2, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, code)
+    for r in range(2):
+        for b in range(-(-lens[r] // BS)):
+            e = SPREADS[spread](b)
+            sc[1, table[r, b]] = 0.0 if e is None else sc[1, table[r, b]] * 2.0 ** e
+    vs = torch.from_numpy(sc[1].astype(np.float32)).to(cuda)
+    pos, req, at = place(cuda, form, lens, rows)
+    if rows > 64:
+        assert tiles_take(N=2 * rows, R=2, H=H, Hkv=Hkv, D=D, W=11, P=20, block_size=BS, window=window or -1, sinks=sinks,
+                          **({} if form == "ragged" else {"rows_per_req": rows}))
+    q = torch.from_numpy(3 * rng.standard_normal((2 * rows, H, D))).to(cuda).to(torch.bfloat16)
+    o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), window=window, sinks=sinks, lse=True,
+                               nsplit=4 if form == "split" else 0, **at)
+    close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, window, sinks, D ** -0.5))

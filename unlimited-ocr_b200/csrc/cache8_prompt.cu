@@ -6,15 +6,18 @@
 //                                 to f16 exactly; q times a power of two (its
 //                                 largest element in [1, 2)) is exact in f16.
 //   z = S * (row factor * kscale) log2 units, per 16-key group (a page's part)
-//   w = 2^(z - m + log2(vscale / vref) + 7)  the softmax weight times the value
-//                                 scale, so that both scales cost nothing per key
-//   O += W D,  l += sum(w) vref / vscale     W rounded to f16; D the value codes
-//   out = O vref / l,  lse = m + log2(l) - 7
-// m is the running maximum, moved only when a row's maximum passes it by 8 (then
-// w stays under 2^15, f16's range); vref follows the largest value scale of a
-// step and moves when that grows or falls by 2^10 to 2^60 (under that a step
-// adds nothing to O), so that a weight under 2^-21 of its row's largest is the
-// first to lose bits.  O is rescaled when either moves.
+//   y = z + log2 vscale
+//   w = 2^(y - my + 7)            the softmax weight times the value scale, so that
+//                                 both scales cost nothing per key
+//   O += W D,  l += sum(w) 2^(my - log2 vscale - mz)     W rounded to f16; D the
+//                                 value codes
+//   out = O 2^(my - mz) / l,  lse = mz + log2(l) - 7
+// mz and my are a row's own running maxima of z and y over the keys that it sees.
+// They move, and l and O are rescaled, when either is passed by 8 (w stays under
+// 2^15, f16's range).  So a key's product of weight and value scale keeps f16's 11
+// bits down to 2^-21 of the row's largest such product, and is off by at most
+// 2^-32 of that below.  Where a page's scale is 2^64 under the others it counts as
+// that: w is 0 in f16 all the same, and l needs its sum.
 //
 // What bounds it: per 128 keys and 256 rows of 128 features, 2048 tensor cycles
 // (4 * 128 * 128 * 256 flops), as many exp2 cycles, and the code conversion
@@ -56,7 +59,9 @@ constexpr int kPrThreads = 416;
 constexpr int kPrConv = 8, kPrMma = 12;  // first warp of the converters, the MMA warp
 constexpr int kPrKeys = 128;             // keys of a step
 constexpr float kPrShift = 7.f;          // weights are kept times 2^7
-constexpr float kPrRescale = 8.f;        // a row's maximum may pass m by this
+constexpr float kPrRescale = 8.f;        // a row's maxima may pass mz and my by this
+constexpr float kPrNoValue = -1e4f;      // log2 of a value scale of 0: adds nothing to any O in fp32
+constexpr float kPrFar = -64.f;          // log2 vscale - (my - mz) from which a group's w is 0 in f16
 constexpr int kPrTmem = 512;
 
 template <int D>
@@ -204,10 +209,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
   __shared__ uint64_t drain_bar;
   // per step, in rings that no reader can be a whole turn behind (the tiles of a
   // pair are at most 3 steps apart): kscale and log2 vscale of its 16-key groups,
-  // groups that exist (bits 0-7), the largest log2 vscale; keys with a NaN value
-  // code, zeroed 4 steps ahead
+  // groups that exist (bits 0-7); keys with a NaN value code, zeroed 4 steps ahead
   __shared__ __align__(16) float g_ks[8][8], g_lv[8][8];
-  __shared__ float g_top[8];
   __shared__ uint32_t g_on[8], g_nan[16][4], g_poison[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
 
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + s * 256 + lane_off, tm_o = tm_s + kO;
-    float m = -INFINITY, l = 0.f, lref = -126.f;  // lref: log2 of vref
+    float m = -INFINITY, dy = 0.f, l = 0.f;  // mz, my - mz
     bool poison = false, ok = true;
     int cnt = 0;
     uint32_t seen[4];   // keys that this row saw of a step seen in part, until its
@@ -335,7 +338,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         return (bit_range(max(p - T.win + 1, 0) - kb, up) | bit_range(0, min(T.sinks - kb, up))) &
                ((on >> (2 * c) & 1 ? 0xffffu : 0u) | (on >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
       };
-      auto group_max = [&](const float* v, int grp) {  // of 16 raw scores, in z units
+      float tz = -INFINITY, ty = -INFINITY;  // the row's largest z and y of this step
+      auto group_max = [&](const float* v, int grp) {  // 16 raw scores
         float x = max3(v[0], v[1], v[2]), y = max3(v[3], v[4], v[5]);
         x = max3(x, v[6], v[7]);
         y = max3(y, v[8], v[9]);
@@ -345,11 +349,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         x = fmaxf(x, y);
         return x == -INFINITY ? x : x * (g_ks[ri][grp] * rowf);
       };
-      // the row's largest score.  WHOLE is compile-time: a run-time test would be
-      // turned into selects on every score
+      // WHOLE is compile-time: a run-time test would be turned into selects on every
+      // score
       auto largest = [&](auto whole_) {
         constexpr bool WHOLE = decltype(whole_)::value;
-        float mx = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < 4; c += 2) {
           float v[32], w[32];
@@ -364,20 +367,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
               w[e] = vb >> e & 1 ? w[e] : -INFINITY;
             }
           }
-          mx = fmaxf(mx, max3(group_max(v, 2 * c), group_max(v + 16, 2 * c + 1), group_max(w, 2 * c + 2)));
-          mx = fmaxf(mx, group_max(w + 16, 2 * c + 3));
+          const float x0 = group_max(v, 2 * c), x1 = group_max(v + 16, 2 * c + 1);
+          const float x2 = group_max(w, 2 * c + 2), x3 = group_max(w + 16, 2 * c + 3);
+          tz = fmaxf(fmaxf(tz, x3), max3(x0, x1, x2));
+          const float* lv = &g_lv[ri][2 * c];
+          ty = fmaxf(fmaxf(ty, x3 + lv[3]), max3(x0 + lv[0], x1 + lv[1], x2 + lv[2]));
         }
-        return mx;
       };
-      const float mx = whole ? largest(std::true_type()) : largest(std::false_type());
-      const float top = g_top[ri];
-      // the same in every thread
-      const bool move_v = on && (top > lref || (top < lref - 10.f && top > lref - 60.f));
-      const bool move_m = mx > m + kPrRescale;
-      if (__any_sync(0xffffffffu, move_m) || move_v) {
-        const float mn = move_m ? mx : m;
-        const float ln = move_v ? top : lref;
-        const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn), alpha_o = alpha * exp2f(lref - ln);
+      if (whole) largest(std::true_type());
+      else largest(std::false_type());
+      const bool move = tz > m + kPrRescale || ty > m + dy + kPrRescale;
+      if (__any_sync(0xffffffffu, move)) {
+        const float nz = move ? fmaxf(m, tz) : m, ny = move ? fmaxf(m + dy, ty) - nz : dy;
+        const float alpha = m == -INFINITY ? 0.f : ex2(m - nz), alpha_o = m == -INFINITY ? 0.f : ex2((m - nz) + (dy - ny));
         if (cnt > 0) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -391,8 +393,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
           tmem_wait_st();
         }
         l *= alpha;
-        m = mn;
-        lref = ln;
+        m = nz;
+        dy = ny;
       }
       const float base = kPrShift - (m == -INFINITY ? 0.f : m);
       // weights of 32 keys -> f16 pairs over their scores' first 16 columns
@@ -403,8 +405,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const int grp = 2 * c + g;
-          float lv = g_lv[ri][grp] - lref;  // the value scale, relative to vref
-          if (lv < -64.f) lv = -64.f;
+          // y - my = z - mz + lv; under kPrFar w is 0 and only the sum counts
+          const float lv = fmaxf(g_lv[ri][grp] - dy, kPrFar);
           const float f = g_ks[ri][grp] * rowf, add = lv + base;
           const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -458,7 +460,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
         check_nan();
         const bool any = l > 0.f || l != l;
         poison = poison || g_poison[s];
-        const float inv = poison ? NAN : any ? exp2f(lref) / l : 0.f;
+        // (2^(my - mz) in two halves: it may pass fp32's range where out does not)
+        const float half = any ? exp2f(0.5f * dy) : 0.f, inv = poison ? NAN : any ? half / l : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = cnt > 0 && (any || poison) ? v[e] * inv : 0.f;
+          for (int e = 0; e < 32; ++e) v[e] = cnt > 0 && (any || poison) ? v[e] * half * inv : 0.f;
           if (active) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) store8(a.out, row * a.s_on + h * a.s_oh + 32 * c + e, a.out_dtype, v + e);
@@ -550,24 +553,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       const uint32_t par = static_cast<uint32_t>(((i >> 1) - 1) & 1);
       const Group g2 = load_group(i + 2);
       if (warp == kPrConv) {
-        float ks = 0.f, lv = -126.f;
+        float ks = 0.f, lv = 0.f;
         if (g0.page >= 0) {
           ks = a.ks[g0.page * a.s_scale + hk];
           lv = log2f(a.vs[g0.page * a.s_scale + hk]);
-          if (lv < -126.f) lv = -126.f;  // a scale of 0 too
+          if (lv < kPrNoValue) lv = kPrNoValue;
         }
         const uint32_t on = __ballot_sync(0xffffffffu, g0.page >= 0) & 0xffu;
-        float top = g0.page >= 0 ? lv : -INFINITY;
-        top = warp_max(top);
         if (lane < 8) {
           g_ks[ri][lane] = ks;
           g_lv[ri][lane] = lv;
         }
         if (lane < 4) g_nan[(i + 4) & 15][lane] = 0;
-        if (lane == 0) {
-          g_on[ri] = on;
-          g_top[ri] = top;
-        }
+        if (lane == 0) g_on[ri] = on;
       }
       if (!__all_sync(0xffffffffu, i < 2 || pr_wait(&k_empty[st], par, abort_p, 621))) break;
       store_tile(sbase + SM::k(st), kx);
