@@ -168,7 +168,8 @@ SPREADS = {"neighbours": lambda b: 30 * (b % 2) - 15, "steps": lambda b: 70 * (b
 
 @pytest.mark.parametrize("spread", list(SPREADS))
 @pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3), (200, 0)])
-@pytest.mark.parametrize("rows,form,code,D", [(300, "rows", "e4m3", 128), (270, "ragged", "int8", 64)])
+@pytest.mark.parametrize("rows,form,code,D", [(300, "rows", "e4m3", 128), (270, "ragged", "int8", 64), (1, "rows", "e4m3", 128),
+                                              (5, "rows", "int8", 64), (1, "split", "e4m3", 64)])
 def test_value_scales_of_any_spread(cuda, spread, window, sinks, rows, form, code, D):
     """Value scales up to 2^200 apart, or 0, from page to page: every row as good
     as its own keys allow, whatever its neighbours see."""
@@ -188,3 +189,27 @@ def test_value_scales_of_any_spread(cuda, spread, window, sinks, rows, form, cod
     o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), window=window, sinks=sinks, lse=True,
                                nsplit=4 if form == "split" else 0, **at)
     close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, window, sinks, D ** -0.5))
+
+
+@pytest.mark.parametrize("nsplit", [0, 1, 2])
+@pytest.mark.parametrize("rows", [1, 6])
+def test_small_weight_on_a_large_scale(cuda, rows, nsplit):
+    """Keys of weight 2^-20 to 2^-60 whose page's value scale makes up for it."""
+    rng = np.random.default_rng(61)
+    lens, H, Hkv, D, BS = [400, 200], 4, 2, 128, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "int8")
+    q = torch.ones(2 * rows, H, D, device=cuda, dtype=torch.bfloat16)
+    kb = np.zeros((sc.shape[1], BS, Hkv, D), np.uint8)
+    for r in range(2):
+        for b in range(-(-lens[r] // BS)):  # every key of block b has the logit -8 b: weight 2^(-11.5 b)
+            kb[table[r, b], :, :, 0] = 256 - b if b else 0
+            sc[0, table[r, b]] = 1.0
+            sc[1, table[r, b]] = 2.0 ** (12 * b)
+    k = torch.from_numpy(kb).to(cuda).view(torch.int8)
+    v = v.contiguous()
+    vals[0] = O8.codes_to_values(kb, "int8")
+    pos, req, at = place(cuda, "rows", lens, rows)
+    ks, vs = (torch.from_numpy(x.astype(np.float32)).to(cuda) for x in sc)
+    o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), lse=True, sm_scale=8.0,
+                               nsplit=nsplit, **at)
+    close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, None, 0, 8.0))

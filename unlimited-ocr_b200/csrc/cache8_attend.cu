@@ -9,8 +9,9 @@
 //   * codes widen to f16 exactly; q is scaled by a power of two so that it is
 //     exact in f16 too (bf16 elements under 2^-28 of the row's largest lose
 //     bits that fp32 sums would not show);
-//   * softmax weights, times 2^15, are rounded to f16 (2^-11 relative down to
-//     2^-29 of a row's largest, where f16 runs out of exponents).
+//   * softmax weights are rounded to f16 times 2^15 and relative to the largest of
+//     their own unit (16 or 32 keys of one page): 2^-11 relative down to 2^-29 of
+//     that, where f16 runs out of exponents, whatever the page's value scale.
 // Both scales are applied in fp32, outside the MMAs.
 //
 // What bounds it: bytes.  A key costs 2 D bytes and 4 D flops per query head,
@@ -45,7 +46,7 @@
 
 namespace srswa {
 
-constexpr float kRowsShift = 15.f;  // weights, their sums and the outputs are kept times 2^15
+constexpr float kRowsShift = 15.f;  // weights, their sums and the outputs are kept times 2^15 (of their unit, or row)
 // Warps of a CTA whose warps share an item: where an SM has one such CTA, and two
 // (of 128 features four warps with room for three units in flight take 18.0 us
 // where six with two take 19.0: 64 requests of 16 / 4 heads, 1024 keys; of 64
@@ -405,16 +406,23 @@ __global__ void __launch_bounds__(32 * NW, NW == alone_warps(D) ? 1 : 2) cache8_
         m0 = n0m;
         m1 = n1m;
       }
-      const float e0 = u0 - kRowsShift, e1 = u1 - kRowsShift;
+      // weights relative to the unit's largest; what that is to the row's comes in
+      // fp32, with the value scale
+      const float a0 = ex2(c0m - u0), a1 = ex2(c1m - u1);
+      const float e0 = (c0m == -INFINITY ? 0.f : c0m) - kRowsShift, e1 = (c1m == -INFINITY ? 0.f : c1m) - kRowsShift;
+      float s0 = 0.f, s1 = 0.f;
       uint32_t pb[CH][2];
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const float p0 = ex2(x[c][0] - e0), p1 = ex2(x[c][1] - e1), p2 = ex2(x[c][2] - e0), p3 = ex2(x[c][3] - e1);
-        l0 += p0 + p2;
-        l1 += p1 + p3;
+        s0 += p0 + p2;
+        s1 += p1 + p3;
         pb[c][0] = transpose8x8(pack_half2(p0, p1));
         pb[c][1] = transpose8x8(pack_half2(p2, p3));
       }
+      l0 = fmaf(s0, a0, l0);
+      l1 = fmaf(s1, a1, l1);
+      const float vs0 = vs * a0, vs1 = vs * a1;
       uint32_t w[CH][4][D / 32];
       load_v(src + CH * CB, w);
       if (!MULTI || whole) {  // masked keys were filled with zeros
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(32 * NW, NW == alone_warps(D) ? 1 : 2) cache8_
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) o[2 * e + u][y] = fmaf(vs, acc[u][y], o[2 * e + u][y]);
+            for (int y = 0; y < 4; ++y) o[2 * e + u][y] = fmaf(y & 1 ? vs1 : vs0, acc[u][y], o[2 * e + u][y]);
         }
       } else {
         // rows of the group see different keys: each takes the unit with the
@@ -447,10 +455,10 @@ __global__ void __launch_bounds__(32 * NW, NW == alone_warps(D) ? 1 : 2) cache8_
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               float* oo = o[2 * e + u];
-              oo[0] = take0 ? fmaf(vs, acc[u][0], oo[0]) : oo[0];
-              oo[1] = take1 ? fmaf(vs, acc[u][1], oo[1]) : oo[1];
-              oo[2] = take0 ? fmaf(vs, acc[u][2], oo[2]) : oo[2];
-              oo[3] = take1 ? fmaf(vs, acc[u][3], oo[3]) : oo[3];
+              oo[0] = take0 ? fmaf(vs0, acc[u][0], oo[0]) : oo[0];
+              oo[1] = take1 ? fmaf(vs1, acc[u][1], oo[1]) : oo[1];
+              oo[2] = take0 ? fmaf(vs0, acc[u][2], oo[2]) : oo[2];
+              oo[3] = take1 ? fmaf(vs1, acc[u][3], oo[3]) : oo[3];
             }
           }
         }
