@@ -729,7 +729,8 @@ SRSWA_API int srswa_rope2d_decode(const int64_t* new_ids, int64_t s_ids, int64_t
  * Rows (query rows of the attend, new tokens of the append) come in two forms:
  *   cu_rows == NULL: row n belongs to request n / rows_per_req, at position
  *     seq_lens[r] - rows_per_req + n % rows_per_req (the last rows of each
- *     request; N = R * rows_per_req);
+ *     request; N = R * rows_per_req; in a request shorter than that the first
+ *     rows' positions are negative: they are not appended, and see nothing);
  *   cu_rows [R + 1]: rows cu_rows[r] <= n < cu_rows[r + 1] belong to request r,
  *     at position prefix_lens[r] + n - cu_rows[r] (varlen, cu_rows ascending).
  *     Rows before cu_rows[0] and from cu_rows[R] on belong to no request: the

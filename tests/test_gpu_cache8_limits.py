@@ -213,3 +213,34 @@ def test_small_weight_on_a_large_scale(cuda, rows, nsplit):
     o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), lse=True, sm_scale=8.0,
                                nsplit=nsplit, **at)
     close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, None, 0, 8.0))
+
+
+@pytest.mark.parametrize("rows", [4, 70])
+@pytest.mark.parametrize("code,real,BS", [("e4m3", "bf16", 64), ("int8", "f32", 16)])
+def test_append_requests_shorter_than_their_rows(cuda, rows, code, real, BS):
+    """The rows at positions 0 and up are written, as the varlen form writes them."""
+    rng = np.random.default_rng(65)
+    lens = [0, 1, 2, 3, 4, 5, 17, 64, 69, 70, 71, 200]
+    R, Hkv, D, W = len(lens), 2, 128, -(-200 // BS)
+    real = {"bf16": torch.bfloat16, "f32": torch.float32}[real]
+    bt = torch.from_numpy(rng.permutation(R * W).astype(np.int32).reshape(R, W)).to(cuda)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    a, b = (cache8.Cache8(R * W, BS, Hkv, D, dtype=CODE[code], device=cuda) for _ in range(2))
+    pre = [max(n - rows, 0) for n in lens]
+    first = torch.from_numpy(rng.standard_normal((2, sum(pre), Hkv, D))).to(cuda).to(real)
+    for c in (a, b):
+        c.append(*first, bt, cu_seqlens=i32([0, *np.cumsum(pre)]), prefix_lens=i32([0] * R))
+    x = torch.from_numpy(rng.standard_normal((2, R * rows, Hkv, D))).to(cuda).to(real)
+    a.append(*x, bt, i32(lens))
+    there = [r * rows + i for r, n in enumerate(lens) for i in range(rows) if n - rows + i >= 0]
+    new = [min(n, rows) for n in lens]
+    b.append(*x[:, there], bt, cu_seqlens=i32([0, *np.cumsum(new)]), prefix_lens=i32(pre))
+    for s, t in zip(a.tensors(), b.tensors()):
+        assert torch.equal(s.view(torch.uint8) if s.dtype != torch.float32 else s, t.view(torch.uint8) if t.dtype != torch.float32 else t)
+    # and both are the definition's
+    vals, sc = np.zeros((R * W, BS, Hkv, D)), np.ones((R * W, Hkv))
+    O8.append(first[0].double().cpu().numpy(), vals, sc, bt.cpu().numpy(), [0] * R, pre, BS, code)
+    O8.append(x[0, there].double().cpu().numpy(), vals, sc, bt.cpu().numpy(), pre, new, BS, code)
+    got = O8.codes_to_values(np.ascontiguousarray(a.k.view(torch.uint8).cpu().numpy()), code)
+    np.testing.assert_array_equal(a.k_scale.double().cpu().numpy(), sc)
+    np.testing.assert_array_equal(got, vals)

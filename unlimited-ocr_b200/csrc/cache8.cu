@@ -139,6 +139,11 @@ __global__ void __launch_bounds__(kAppendThreads, 6) cache8_append_kernel(const 
     n = a.rows.rps;
     row0 = req * n;
     start = static_cast<int64_t>(a.rows.seq_lens[req]) - n;
+    if (start < 0) {  // a request shorter than its rows: the first of them have no position
+      row0 -= start;
+      n += start;
+      start = 0;
+    }
   }
   if (n <= 0 || start < 0 || row0 < 0 || row0 + n > a.N) return;
   const int64_t blk = start / a.BS + nth;
