@@ -368,7 +368,8 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
 }
 
 extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen) {
-  if (!d || d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0 || d->rows_per_req <= 0) return 0;
+  if (!d || d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0) return 0;
+  if (!varlen && d->rows_per_req <= 0) return 0;
   if (prompt_applies(*d, varlen != 0)) return 16;  // the status word
   return rows_plan(*d, varlen != 0).bytes;
 }
