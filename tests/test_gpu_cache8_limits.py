@@ -244,3 +244,23 @@ def test_append_requests_shorter_than_their_rows(cuda, rows, code, real, BS):
     got = O8.codes_to_values(np.ascontiguousarray(a.k.view(torch.uint8).cpu().numpy()), code)
     np.testing.assert_array_equal(a.k_scale.double().cpu().numpy(), sc)
     np.testing.assert_array_equal(got, vals)
+
+
+@pytest.mark.parametrize("qs", [2.0 ** -100, 2.0 ** -40, 1.0, 2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("code,D", [("e4m3", 128), ("int8", 64)])
+@pytest.mark.parametrize("rows", [300, 5])
+def test_query_range(cuda, qs, code, D, rows):
+    """bf16 queries of any magnitude, and one element 2^20 above the rest on a
+    feature that the keys leave at 0."""
+    rng = np.random.default_rng(63)
+    lens, H, Hkv, BS = [700, 350], 8, 2, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, code)
+    k.view(torch.uint8)[..., 5] = 0
+    vals[0, ..., 5] = 0
+    pos, req, at = place(cuda, "rows", lens, rows)
+    q = (torch.from_numpy(rng.standard_normal((2 * rows, H, D))) * qs).to(torch.bfloat16)
+    q[..., 5] = 2.0 ** 20 * qs
+    q = q.to(cuda)
+    sm = D ** -0.5 / qs
+    o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), lse=True, sm_scale=sm, **at)
+    close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, None, 0, sm))

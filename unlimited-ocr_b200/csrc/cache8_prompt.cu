@@ -3,8 +3,9 @@
 //
 // Mathematics, per query head, for the rows of a tile and 128 keys at a time:
 //   S = Q C^T                     f16 operands, fp32 in TMEM.  The codes C widen
-//                                 to f16 exactly; q times a power of two (its
-//                                 largest element in [1, 2)) is exact in f16.
+//                                 to f16 exactly, and so does q times a power of
+//                                 two (its largest element in [2^14, 2^15); bf16
+//                                 elements under 2^-31 of that lose bits).
 //   z = S * (row factor * kscale) log2 units, per 16-key group (a page's part)
 //   y = z + log2 vscale
 //   w = 2^(y - my + 7)            the softmax weight times the value scale, so that
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
           mx = fmaxf(mx, fmaxf(fabsf(x), fabsf(y)));
         }
       }
-      int e2 = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+      int e2 = static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 14;
       e2 = mx == 0.f ? 0 : max(min(e2, 126), -126);
       float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
       rowf = __uint_as_float(static_cast<uint32_t>(127 + e2) << 23) * fabsf(a.scale_log2);
