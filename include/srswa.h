@@ -770,9 +770,10 @@ SRSWA_API int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, con
  * without a bias, and the other keys j <= p of its selected blocks topk_idx
  * [(Hkv,) N, K] (int32 / int64; ids outside [0, W) unused, a repeated id counts
  * once) with the slot's bias (fp32, same layout, or NULL).  Softmax of
- * sm_scale * q . k + bias over them; out [N, H, D] (out_dtype: q's type or F32)
- * and lse_out [N, H] fp32 natural log (optional).  A row that sees nothing
- * gives 0 and -inf.  Codes of keys that a row does not see never reach its
+ * sm_scale * q . k + bias over them (in fp32 log2 units: a finite bias beyond
+ * +-2.35e38 counts as that; keys with one of -inf weigh 0); out [N, H, D]
+ * (out_dtype: q's type or F32) and lse_out [N, H] fp32 natural log (optional).
+ * A row that sees nothing, or no key of any weight, gives 0 and -inf.  Codes of keys that a row does not see never reach its
  * result, whatever they hold; NaN in those that it sees does.  workspace:
  * srswa_cache8_attend_workspace_size bytes, 16-byte aligned (0: none).  Calls
  * with many rows per request go to tensor-core tiles: their workspace is 16

@@ -264,3 +264,39 @@ def test_query_range(cuda, qs, code, D, rows):
     sm = D ** -0.5 / qs
     o, lse = ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), lse=True, sm_scale=sm, **at)
     close(o, lse, dense(q.double().cpu().numpy(), vals, sc, table, req, pos, None, 0, sm))
+
+
+@pytest.mark.parametrize("low", [-3.4028234663852886e38, -3e38, -1e38, 3.4028234663852886e38])
+@pytest.mark.parametrize("nsplit", [0, 3])
+def test_bias_at_the_end_of_its_type(cuda, low, nsplit):
+    """Selected blocks all at the lowest value: the row still weighs them (by the
+    bias, which swallows the scores); beside keys of the window they weigh
+    nothing.  lse is held in log2 units: a bias past 2^128 ln 2 counts as that."""
+    rng = np.random.default_rng(64)
+    lens, H, Hkv, D, BS = [512, 700], 4, 2, 128, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    q = torch.from_numpy(rng.standard_normal((2, H, D))).to(cuda).to(torch.bfloat16)
+    topk = torch.tensor([[0, 2, 3], [1, 4, -1]], dtype=torch.int32, device=cuda)
+    bias = torch.full((2, 3), low, device=cuda)
+    lens_t, bt = torch.tensor(lens, dtype=torch.int32, device=cuda), torch.from_numpy(table).to(cuda)
+    run = lambda w, b: ops.cache8_attend(q, k, v, ks, vs, bt, lens_t, window=w, topk_idx=topk, bias=b, lse=True,  # noqa: E731
+                                         nsplit=nsplit)
+    o, lse = run(0, bias)
+    assert torch.isfinite(o).all()
+    g = lse.double().cpu().numpy()
+    end = math.copysign(min(abs(low), 3.4028234663852886e38 * math.log(2)), low)
+    assert np.abs(g / end - 1).max() <= 1e-6
+    for r in range(2):
+        pages = table[r, [b for b in topk[r].tolist() if b >= 0]]
+        for h in range(H):
+            val = (vals[1, pages, :, h // 2] * sc[1, pages, h // 2][:, None, None]).reshape(-1, D)
+            got = o[r, h].double().cpu().numpy()
+            assert (np.abs(got - val.mean(0)) <= 2.0 ** -8 * np.abs(val.mean(0)) + 2.0 ** -10 * np.abs(val).mean(0)).all()
+    if low < 0:
+        near = ops.cache8_attend(q, k, v, ks, vs, bt, lens_t, window=100, lse=True, nsplit=nsplit)
+        both = run(100, bias)
+        ref = dense(q.double().cpu().numpy(), vals, sc, table, np.arange(2), np.array(lens) - 1, 100, 0, D ** -0.5)
+        close(*both, ref)
+        close(*near, ref)
+    masked = run(0, torch.full((2, 3), -math.inf, device=cuda))
+    assert (masked[0] == 0).all() and torch.isneginf(masked[1]).all()

@@ -171,7 +171,10 @@ __global__ void __launch_bounds__(32 * NW, NW == alone_warps(D) ? 1 : 2) cache8_
         int64_t b = -1;
         if (si >= 0 && si < K) {
           b = load_index(a.sel, ib + si, a.idx_is64);
-          if (a.bias) r.b2 = a.bias[hk * a.s_b_h + n0 * a.s_b_n + si] * kLog2e;
+          if (a.bias) {  // (the ends of fp32 stay finite: such a mask is not -inf)
+            const float b0 = a.bias[hk * a.s_b_h + n0 * a.s_b_n + si];
+            r.b2 = fabsf(b0) < INFINITY ? fminf(fmaxf(b0 * kLog2e, -3.402823466e38f), 3.402823466e38f) : b0;
+          }
         }
         bool once = b >= 0 && b < a.W;
         const int upto = min(first + 31 - n_fix, K - 1);  // the last selected slot of this block
