@@ -20,3 +20,23 @@ def test_varlen_workspace_needs_no_rows_per_req(kw, some):
     assert workspace(1, rows_per_req=0, **kw) == want
     assert workspace(0, rows_per_req=0, **kw) == 0
     assert (want > 0) == some
+
+
+END = 2 ** 63 - 1
+
+
+@pytest.mark.parametrize("varlen,kw", [(0, {}), (0, dict(W=4000)), (0, dict(W=4000, K=8)), (1, dict(N=900, W=200))])
+def test_plans_at_the_end_of_the_arguments(varlen, kw):
+    """Windows, sinks and part counts of any size are as good as all there is."""
+    assert workspace(varlen, window=END, **kw) == workspace(varlen, window=-1, **kw)
+    assert workspace(varlen, window=END, sinks=END, **kw) == workspace(varlen, window=-1, **kw)
+    assert workspace(varlen, window=512, sinks=END, **kw) == workspace(varlen, window=512, sinks=2 ** 30, **kw)
+    parts = (kw.get("W", 5) + kw.get("K", 0)) * 2  # units of 32 keys in pages of 64
+    for n in (2 ** 62, 2 ** 62 + 1, END):
+        assert 0 < workspace(varlen, nsplit=n, **kw) == workspace(varlen, nsplit=parts, **kw)
+
+
+def test_refusals_of_sizes():
+    d = lambda **kw: L.lib().srswa_cache8_attend(C.byref(desc(**kw)), *[1 << 20] * 6, 1 << 20, None, None, 1 << 20, None,  # noqa: E731
+                                                 1 << 20, None, None, 0, None)
+    assert d(K=513) == d(K=END) == d(W=1 << 31) == d(P=1 << 31) == L.ETOOLARGE

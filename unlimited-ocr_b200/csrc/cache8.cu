@@ -319,7 +319,7 @@ static int check_common(const srswa_cache8_desc* d, const int32_t* seq_lens, con
   SRSWA_CHECK_ARG(d->N >= 0 && d->R >= 0 && d->Hkv > 0 && d->P >= 0 && d->W >= 0 && d->block_size > 0, SRSWA_EINVAL);
   SRSWA_CHECK_ARG(kv_code_ok(d->kv_dtype) && (d->D == 64 || d->D == 128), SRSWA_EUNSUPPORTED);
   SRSWA_CHECK_ARG(d->block_size % 16 == 0, SRSWA_EUNSUPPORTED);
-  SRSWA_CHECK_ARG(d->block_size <= 1024 && d->Hkv <= 65535, SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(d->block_size <= 1024 && d->Hkv <= 65535 && d->W < (1ll << 31) && d->P < (1ll << 31), SRSWA_ETOOLARGE);
   SRSWA_CHECK_ARG(((d->s_page | d->s_pos | d->s_head) & 15) == 0, SRSWA_EALIGN);
   if (cu_rows) {
     SRSWA_CHECK_ARG(prefix_lens, SRSWA_EINVAL);
@@ -367,25 +367,37 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
   return d->kv_dtype == SRSWA_I8 ? append_start<64, SRSWA_I8>(a, slots, st) : append_start<64, SRSWA_F8E4M3>(a, slots, st);
 }
 
-extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen) {
-  if (!d || d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0) return 0;
+// Positions are 32-bit: a window or sinks past them are all there is.
+static srswa_cache8_desc within_positions(const srswa_cache8_desc* d) {
+  constexpr int64_t all = 0x7ffffe00;
+  srswa_cache8_desc c = *d;
+  if (c.window > all) c.window = all;
+  if (c.sinks > all) c.sinks = all;
+  return c;
+}
+
+extern "C" size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* desc, int varlen) {
+  if (!desc) return 0;
+  const srswa_cache8_desc bounded = within_positions(desc), *d = &bounded;
+  if (d->N <= 0 || d->Hkv <= 0 || d->H <= 0 || d->H % d->Hkv || d->block_size <= 0) return 0;
   if (!varlen && d->rows_per_req <= 0) return 0;
   if (prompt_applies(*d, varlen != 0)) return 16;  // the status word
   return rows_plan(*d, varlen != 0).bytes;
 }
 
-extern "C" int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, const void* k_cache,
+extern "C" int srswa_cache8_attend(const srswa_cache8_desc* desc, const void* q, const void* k_cache,
                                    const void* v_cache, const float* k_scale, const float* v_scale,
                                    const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_rows,
                                    const int32_t* prefix_lens, const void* topk_idx, const float* bias, void* out,
                                    float* lse_out, void* workspace, size_t workspace_bytes, srswa_stream_t stream) {
-  SRSWA_CHECK_ARG(d, SRSWA_EINVAL);
+  SRSWA_CHECK_ARG(desc, SRSWA_EINVAL);
+  const srswa_cache8_desc bounded = within_positions(desc), *d = &bounded;
   const int rc = check_common(d, seq_lens, cu_rows, prefix_lens);
   if (rc) return rc;
   SRSWA_CHECK_ARG(d->H > 0 && d->H % d->Hkv == 0 && d->K >= 0 && d->sinks >= 0, SRSWA_EINVAL);
   SRSWA_CHECK_ARG(d->q_dtype == SRSWA_BF16 || d->q_dtype == SRSWA_F16, SRSWA_EUNSUPPORTED);
   SRSWA_CHECK_ARG(d->out_dtype == d->q_dtype || d->out_dtype == SRSWA_F32, SRSWA_EUNSUPPORTED);
-  SRSWA_CHECK_ARG(d->H <= 65535 && d->N < (1ll << 31), SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(d->H <= 65535 && d->N < (1ll << 31) && d->K <= kMaxSelected, SRSWA_ETOOLARGE);
   if (d->N == 0) return SRSWA_OK;
   SRSWA_CHECK_ARG(q && k_cache && v_cache && k_scale && v_scale && block_table && out, SRSWA_EINVAL);
   SRSWA_CHECK_ARG(d->K == 0 || topk_idx, SRSWA_EINVAL);

@@ -57,7 +57,6 @@ constexpr int pair_warps(int D) { return D == 128 ? 4 : 6; }
 // are no faster, and eight warps an SM with 24 KB each beat twelve with 16 KB
 // at D = 128: 134.5 and 139 us for the 750 MB of six requests of 30k to 131k keys).
 constexpr int ring_bytes(int D) { return D == 128 ? 24576 : 8192; }
-constexpr int kMaxSelected = 512;
 constexpr int kCols = 8;  // queries that share a pass over the keys (columns of the MMA)
 
 // The keys a row group can see, as slots of one page each: sinks, window,
@@ -735,8 +734,9 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
   p.units = p.items * most;
   const int64_t wave = slots / kRowsWarps;  // CTAs of four warps at a time
   if (d.nsplit > 0) {
-    if (d.nsplit > 1) p.split = kSplitEqual;
-    parts = d.nsplit * p.items;
+    const int64_t n = d.nsplit < most ? d.nsplit : most > 1 ? most : 1;  // a unit each at least
+    if (n > 1) p.split = kSplitEqual;
+    parts = n * p.items;
   } else {
     // The three ways, in us for n requests of 16 / 4 heads of 128 and L keys (4 n
     // items of L / 32 units; one warp each, a CTA each, equal parts):
@@ -794,7 +794,7 @@ static int rows_start(const Attend8Args& a, unsigned ctas, cudaStream_t st) {
 }
 
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st) {
-  if (a.K > kMaxSelected || p.ctas >= (1ll << 28)) return SRSWA_ETOOLARGE;
+  if (p.ctas >= (1ll << 28)) return SRSWA_ETOOLARGE;
   a.share = p.share;
   a.ngrp = p.ngrp;
   a.split = p.split;

@@ -79,6 +79,7 @@ struct RowsPlan {
 };
 constexpr int kRowsWarps = 4;  // of a CTA of the row kernel (plan.warps may be more), and CTAs an SM holds
 constexpr int kRowsCtasPerSm = 2;
+constexpr int kMaxSelected = 512;  // selected blocks of a row
 int sm_count();
 RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen);
 int rows_launch(Attend8Args a, const RowsPlan& p, int kv_dtype, void* workspace, cudaStream_t st);
