@@ -300,3 +300,27 @@ def test_bias_at_the_end_of_its_type(cuda, low, nsplit):
         close(*near, ref)
     masked = run(0, torch.full((2, 3), -math.inf, device=cuda))
     assert (masked[0] == 0).all() and torch.isneginf(masked[1]).all()
+
+
+@pytest.mark.parametrize("rows,form", [(300, "rows"), (257, "ragged"), (64, "ragged")])
+@pytest.mark.parametrize("window", [None, 70])
+def test_nan_value_code_of_the_last_key(cuda, rows, form, window):
+    """It reaches the request's last row alone, in the last step of its tile."""
+    rng = np.random.default_rng(68)
+    lens, H, Hkv, D, BS = [700, 350], 8, 2, 128, 64
+    lens, R = lens * 4, 8
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    pos, req, at = place(cuda, form, lens, rows)
+    assert tiles_take(N=R * rows, R=R, H=H, Hkv=Hkv, D=D, W=11, P=80, block_size=BS, window=window or -1,
+                      **({} if form == "ragged" else {"rows_per_req": rows}))
+    q = torch.from_numpy(rng.standard_normal((R * rows, H, D))).to(cuda).to(torch.bfloat16)
+    run = lambda: ops.cache8_attend(q, k, v, ks, vs, torch.from_numpy(table).to(cuda), window=window, **at)  # noqa: E731
+    clean = run()
+    for r in range(R):
+        j = lens[r] - 1
+        v.view(torch.uint8)[int(table[r, j // BS]), j % BS, :, 9] = 0xFF
+    o = run()
+    last = torch.zeros(R * rows, dtype=torch.bool, device=cuda)
+    last[rows - 1:: rows] = True
+    assert torch.isnan(o[last][:, :, 9]).all()
+    assert torch.equal(o[~last], clean[~last])

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       mbar_init(&q_full[s], 128);
       mbar_init(&s_full[s], 2);  // the MMAs, and the issuing thread's own release of what it saw
       mbar_init(&p_full[s], 128);
-      mbar_init(&o_full[s], 1);
+      mbar_init(&o_full[s], 2);  // likewise: the last step's NaN words are read behind it
       mbar_init(&k_full[s], 128);
       mbar_init(&v_full[s], 128);
       mbar_init(&k_empty[s], 1);
@@ -640,7 +640,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) cache8_prompt_kernel(const Atte
       for (int x = 0; x < kPrKeys / 16; ++x)
         mma_bf16_ts(tmem + s * 256 + kO, tmem + s * 256 + x * 8, vd + x * 128u, id, cnt[s] > 0 || x > 0 ? 1u : 0u);
       ++cnt[s];
-      if (i == last[s]) mma_commit(&o_full[s]);
+      if (i == last[s]) {
+        mma_commit(&o_full[s]);
+        pr_arrive(&o_full[s]);
+      }
       return true;
     };
     if (T.n_steps > 0) {
