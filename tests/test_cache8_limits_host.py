@@ -40,3 +40,30 @@ def test_refusals_of_sizes():
     d = lambda **kw: L.lib().srswa_cache8_attend(C.byref(desc(**kw)), *[1 << 20] * 6, 1 << 20, None, None, 1 << 20, None,  # noqa: E731
                                                  1 << 20, None, None, 0, None)
     assert d(K=513) == d(K=END) == d(W=1 << 31) == d(P=1 << 31) == L.ETOOLARGE
+
+
+def lone(**kw):
+    """Tensors whose dimensions of one element have odd strides."""
+    import torch
+    def odd(t, dim, stride):
+        s = list(t.stride())
+        s[dim] = stride
+        return t.as_strided(t.shape, s)
+    P, BS, D, R = 5, 64, 128, 1
+    k, v = (torch.zeros(P, BS, 1, D, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    q = torch.zeros(1, 1, D, dtype=torch.bfloat16)
+    a = dict(q=odd(odd(q, 0, 3), 1, 5), k=odd(k, 2, 7), v=odd(v, 2, 9), ks=odd(torch.ones(P, 1), 1, 3), vs=torch.ones(P, 1),
+             bt=odd(torch.zeros(R, 4, dtype=torch.int32), 0, 1), lens=torch.ones(1, dtype=torch.int32))
+    a.update(kw)
+    return [a[x] for x in ("q", "k", "v", "ks", "vs", "bt", "lens")]
+
+
+def test_strides_of_single_elements_do_not_count():
+    """One row, one head, one request: their strides are never used.  (The call
+    then stops at the CPU tensors.)"""
+    from srswa import ops
+    with pytest.raises(L.SrswaError, match="CUDA"):
+        ops.cache8_attend(*lone())
+    q, k, v, ks, vs, bt, lens = lone()
+    with pytest.raises(L.SrswaError, match="CUDA"):
+        ops.cache8_append(q, q, k, v, ks, vs, bt, lens)

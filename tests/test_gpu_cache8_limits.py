@@ -324,3 +324,32 @@ def test_nan_value_code_of_the_last_key(cuda, rows, form, window):
     last[rows - 1:: rows] = True
     assert torch.isnan(o[last][:, :, 9]).all()
     assert torch.equal(o[~last], clean[~last])
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_strides_of_single_elements(cuda, rows):
+    """One head, one request: strides that are never used may have any value."""
+    rng = np.random.default_rng(69)
+    n, D, BS = 400, 128, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, [n], 1, D, BS, "int8")
+
+    def odd(t, dim, stride):
+        s = list(t.stride())
+        s[dim] = stride
+        return t.as_strided(t.shape, s)
+    q = torch.from_numpy(rng.standard_normal((rows, 1, D))).to(cuda).to(torch.bfloat16)
+    bt, sl = torch.from_numpy(table).to(cuda), torch.tensor([n], dtype=torch.int32, device=cuda)
+    want = ops.cache8_attend(q, k, v, ks, vs, bt, sl)
+    q1, k1, v1 = odd(q, 1, 5), odd(k, 2, 7), odd(v, 2, 9)
+    if rows == 1:
+        q1 = odd(q1, 0, 3)
+    assert torch.equal(want, ops.cache8_attend(q1, k1, v1, odd(ks, 1, 3), vs, odd(bt, 0, 1), sl, out=odd(torch.empty_like(q), 1, 3)))
+    a, b = k.clone(), k.clone()
+    ops.cache8_append(q, q, a, v.clone(), ks.clone(), vs.clone(), bt, sl)
+    ops.cache8_append(q1, q1, odd(b, 2, 7), odd(v.clone(), 2, 1), odd(ks.clone(), 1, 3), vs.clone(), odd(bt, 0, 1), sl)
+    assert torch.equal(a, b)
+    refs = torch.zeros(len(ks), dtype=torch.int32, device=cuda)
+    refs[bt[0].long()] = 1
+    t1, r1, n1 = ops.pages_compact(bt, refs, [ks])
+    t2, r2, n2 = ops.pages_compact(odd(bt, 0, 1), refs, [ks.clone()])
+    assert torch.equal(t1, t2) and torch.equal(r1, r2) and torch.equal(n1, n2)

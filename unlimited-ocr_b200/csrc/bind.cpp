@@ -88,6 +88,9 @@ bool vector_i32(const at::Tensor& t, const at::Device& dev) {
   return t.scalar_type() == at::kInt && t.dim() == 1 && (t.size(0) <= 1 || t.stride(0) == 1) && t.device() == dev;
 }
 
+// The stride of a dimension of one element (`one`) is never used, whatever it is.
+int64_t step(const at::Tensor& t, int64_t dim, int64_t one = 0) { return t.size(dim) == 1 ? one : t.stride(dim); }
+
 // What append and attend share: the cache, the table and the row form.
 struct Cache {
   srswa_cache8_desc d = {};
@@ -104,25 +107,26 @@ struct Cache {
       value_error("k_cache and v_cache must be [pages, block_size, kv heads, head dim] of one type");
     d.kv_dtype = code_type(*k);
     d.q_dtype = real_type(x);
-    if (v->strides() != k->strides() || k->stride(3) != 1)
+    d.s_page = step(*k, 0);
+    d.s_pos = step(*k, 1);
+    d.s_head = step(*k, 2);
+    if (step(*v, 0) != d.s_page || step(*v, 1) != d.s_pos || step(*v, 2) != d.s_head || step(*k, 3, 1) != 1 ||
+        step(*v, 3, 1) != 1)
       value_error("k_cache and v_cache must share their strides, features contiguous");
     d.P = k->size(0);
     d.block_size = k->size(1);
     d.Hkv = k->size(2);
     d.D = k->size(3);
-    d.s_page = k->stride(0);
-    d.s_pos = k->stride(1);
-    d.s_head = k->stride(2);
+    d.s_scale = step(*ks, 0);
     for (const at::Tensor* s : {ks, vs})
       if (s->dim() != 2 || s->size(0) != d.P || s->size(1) != d.Hkv || s->scalar_type() != at::kFloat ||
-          (s->stride(1) != 1 && d.Hkv > 1) || s->stride(0) != ks->stride(0))
+          step(*s, 1, 1) != 1 || step(*s, 0) != d.s_scale)
         value_error("k_scale and v_scale must be [pages, kv heads] fp32 with one row stride, heads contiguous");
-    d.s_scale = ks->stride(0);
     if (!rows_contiguous(*bt) || bt->scalar_type() != at::kInt)
       value_error("block_table must be [requests, blocks] int32 with contiguous rows");
     d.R = bt->size(0);
     d.W = bt->size(1);
-    d.s_bt = bt->stride(0);
+    d.s_bt = step(*bt, 0);
     if (x.dim() < 1) value_error("rows must be [rows, heads, head dim]");
     d.N = x.size(0);
     d.rows_per_req = 1;
@@ -168,10 +172,10 @@ PyObject* append(PyObject* const* a) {
   if (v.stride(2) != 1) v = v.contiguous();
   d.H = d.Hkv;
   d.out_dtype = d.q_dtype;
-  d.s_qn = k.stride(0);
-  d.s_qh = k.stride(1);
-  d.s_on = v.stride(0);
-  d.s_oh = v.stride(1);
+  d.s_qn = step(k, 0);
+  d.s_qh = step(k, 1);
+  d.s_on = step(v, 0);
+  d.s_oh = step(v, 1);
   check(p_srswa_cache8_append(&d, k.data_ptr(), v.data_ptr(), c.k->data_ptr(), c.v->data_ptr(),
                               static_cast<float*>(c.ks->data_ptr()), static_cast<float*>(c.vs->data_ptr()),
                               static_cast<const int32_t*>(c.bt->data_ptr()), c.lens, c.cu, c.pre, stream_of(k)),
@@ -242,10 +246,10 @@ PyObject* attend(PyObject* const* a) {
   at::Tensor lse;
   if (with_lse) lse = at::empty({d.N, d.H}, q.options().dtype(at::kFloat));
   d.out_dtype = real_type(out);
-  d.s_qn = q.stride(0);
-  d.s_qh = q.stride(1);
-  d.s_on = out.stride(0);
-  d.s_oh = out.stride(1);
+  d.s_qn = step(q, 0);
+  d.s_qh = step(q, 1);
+  d.s_on = step(out, 0);
+  d.s_oh = step(out, 1);
   at::Tensor ws;
   const size_t need = p_srswa_cache8_attend_workspace_size(&d, c.cu != nullptr);
   if (given(a[17])) {
@@ -288,7 +292,7 @@ struct Pool {
       value_error("block_table must be [rows, blocks] int32 with contiguous rows");
     R = bt.size(0);
     W = bt.size(1);
-    s_bt = bt.stride(0);
+    s_bt = step(bt, 0, W);
     if (seq_lens) {
       const at::Tensor& t = tensor(seq_lens, "seq_lens");
       vector(t, "seq_lens");
@@ -418,7 +422,7 @@ PyObject* pages_compact(PyObject* const* a) {
   const size_t need = p_srswa_pages_compact_workspace_size(p.P);
   at::Tensor live = at::empty({1}, i32(p.dev)), ws = at::empty({static_cast<int64_t>(need / 4)}, i32(p.dev));
   check(p_srswa_pages_compact(p.table, p.s_bt, p.R, p.W, p.refs, p.P, t.data(), static_cast<int64_t>(t.size()),
-                              ot.data_ptr<int32_t>(), ot.stride(0), orf.data_ptr<int32_t>(), live.data_ptr<int32_t>(),
+                              ot.data_ptr<int32_t>(), step(ot, 0, p.W), orf.data_ptr<int32_t>(), live.data_ptr<int32_t>(),
                               ws.data_ptr(), need, stream_of(bt)),
         "srswa_pages_compact");
   PyObject *x = THPVariable_Wrap(ot), *y = THPVariable_Wrap(orf), *z = THPVariable_Wrap(live);
