@@ -67,3 +67,11 @@ def test_strides_of_single_elements_do_not_count():
     q, k, v, ks, vs, bt, lens = lone()
     with pytest.raises(L.SrswaError, match="CUDA"):
         ops.cache8_append(q, q, k, v, ks, vs, bt, lens)
+
+
+def test_block_size_past_32_bits_is_refused():
+    lib, X = L.lib(), 1 << 20
+    for bs in (1 << 31, END):
+        assert lib.srswa_pages_free(X, 1, X, 4, 4, 4, X, X, 8, bs, None) == L.ETOOLARGE
+        assert lib.srswa_pages_extend(X, X, 1, X, 4, 4, 4, X, X, 8, bs, X, X, 1 << 30, None) == L.ETOOLARGE
+        assert lib.srswa_pages_fork(X, X, 1, X, 4, 4, 4, X, X, 8, bs, None, 0, X, X, 1 << 30, None) == L.ETOOLARGE

@@ -379,7 +379,7 @@ extern "C" int srswa_pages_free(const int32_t* rows, int64_t n, int32_t* block_t
   const int rc = check_pool(block_table, s_bt, R, W, refs, P);
   if (rc) return rc;
   SRSWA_CHECK_ARG(n >= 0 && block_size > 0 && seq_lens && (n == 0 || rows), SRSWA_EINVAL);
-  SRSWA_CHECK_ARG(n < (1ll << 31), SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(n < (1ll << 31) && block_size < (1ll << 31), SRSWA_ETOOLARGE);
   if (n == 0) return SRSWA_OK;
   return launch_pdl(pages_free_kernel, dim3(static_cast<unsigned>(n)), 256, 0, reinterpret_cast<cudaStream_t>(stream),
                     rows, block_table, s_bt, R, W, seq_lens, refs, P, block_size);
@@ -392,7 +392,7 @@ extern "C" int srswa_pages_extend(const int32_t* rows, const int32_t* new_lens, 
   int rc = check_pool(block_table, s_bt, R, W, refs, P);
   if (rc) return rc;
   SRSWA_CHECK_ARG(n >= 0 && block_size > 0 && seq_lens && short_out && (n == 0 || (rows && new_lens)), SRSWA_EINVAL);
-  SRSWA_CHECK_ARG(n <= 65535, SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(n <= 65535 && block_size < (1ll << 31), SRSWA_ETOOLARGE);
   PlanArgs a = {rows, nullptr, new_lens, n, block_table, s_bt, R, W, P, block_size, seq_lens, refs, short_out};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   rc = make_plan(a, workspace, workspace_bytes, st);
@@ -407,7 +407,7 @@ extern "C" int srswa_pages_fork(const int32_t* parents, const int32_t* children,
   int rc = check_pool(block_table, s_bt, R, W, refs, P);
   if (rc) return rc;
   SRSWA_CHECK_ARG(n >= 0 && block_size > 0 && seq_lens && short_out && (n == 0 || (parents && children)), SRSWA_EINVAL);
-  SRSWA_CHECK_ARG(n <= 65535, SRSWA_ETOOLARGE);
+  SRSWA_CHECK_ARG(n <= 65535 && block_size < (1ll << 31), SRSWA_ETOOLARGE);
   PageTensors pt = {};
   rc = page_tensors(tensors, ntensors, pt);
   if (rc) return rc;
