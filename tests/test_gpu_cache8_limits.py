@@ -20,8 +20,8 @@ import torch
 
 from oracle import cache8 as O8
 from srswa import _lib as L
-from srswa import cache8, ops
-from test_gpu_cache8 import CODE, U, make_cache
+from srswa import cache8, ops, paged
+from test_gpu_cache8 import CODE, U, check, make_cache
 from test_gpu_cache8_forms import tiles_take
 
 pytestmark = pytest.mark.gpu
@@ -353,3 +353,90 @@ def test_strides_of_single_elements(cuda, rows):
     t1, r1, n1 = ops.pages_compact(bt, refs, [ks])
     t2, r2, n2 = ops.pages_compact(odd(bt, 0, 1), refs, [ks.clone()])
     assert torch.equal(t1, t2) and torch.equal(r1, r2) and torch.equal(n1, n2)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("direct", [True, False])
+def test_routed_blocks(cuda, rows, direct):
+    """The decode router's selection and bias (paged.route_decode), taken as they
+    are, next to the local window."""
+    rng = np.random.default_rng(70)
+    lens, H, Hkv, D, BS, local, topk = [900, 70, 2500, 5], 10, 10, 128, 64, 2, 4
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    bt, sl = torch.from_numpy(table).to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    idx_q = torch.from_numpy(rng.standard_normal((len(lens) * rows, 128))).to(cuda).to(torch.bfloat16)
+    k_bar = torch.from_numpy(rng.standard_normal((len(ks), 128)).astype(np.float32)).to(cuda)
+    width = topk if direct else topk + 3
+    out_idx = torch.full((len(lens) * rows, width), 7, dtype=torch.int32, device=cuda)
+    out_bias = torch.full((len(lens) * rows, width), 7.0, device=cuda)
+    paged.route_decode(idx_q=idx_q, k_bar=k_bar, block_table=bt, seq_lens=sl, image_allow=None, out_idx=out_idx,
+                       out_bias=out_bias, max_block=table.shape[1], block_size=BS, local_blocks=local,
+                       decode_query_len=rows, idx_scale=128 ** 0.5, prior_floor=1e-4, sigma=1.0, topm=8, budget=topk)
+    assert (out_idx >= 0).any() and (out_bias != 0).any()
+    q = torch.from_numpy(rng.standard_normal((len(lens) * rows, H, D))).to(cuda).to(torch.bfloat16)
+    o, lse = ops.cache8_attend(q, k, v, ks, vs, bt, sl, window=local * BS, topk_idx=out_idx, bias=out_bias, lse=True)
+    pos, req, _ = place(cuda, "rows", lens, rows)
+    ref = O8.attend(q.double().cpu().numpy(), vals[0], vals[1], sc[0], sc[1], table, req, pos, local * BS, 0,
+                    out_idx.cpu().numpy()[None], out_bias.double().cpu().numpy()[None], D ** -0.5)
+    check(o, lse, ref, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("form", ["rows", "ragged"])
+def test_tiles_in_a_graph(cuda, form):
+    """The tiles' call inside a CUDA graph: lengths are read on the device, and the
+    status word is cleared by each replay."""
+    rng = np.random.default_rng(71)
+    lens, rows, H, Hkv, D, BS = [700, 350], 300, 8, 2, 128, 64
+    k, v, ks, vs, table, vals, sc = make_cache(rng, cuda, lens, Hkv, D, BS, "e4m3")
+    _, _, at = place(cuda, form, lens, rows)
+    assert tiles_take(N=2 * rows, R=2, H=H, Hkv=Hkv, D=D, W=11, P=20, block_size=BS,
+                      **({} if form == "ragged" else {"rows_per_req": rows}))
+    q = torch.from_numpy(rng.standard_normal((2 * rows, H, D))).to(cuda).to(torch.bfloat16)
+    bt, ws = torch.from_numpy(table).to(cuda), torch.full((16,), 255, dtype=torch.uint8, device=cuda)
+    run = lambda: ops.cache8_attend(q, k, v, ks, vs, bt, lse=True, workspace=ws, **at)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, lse = run()
+    for n in (lens, [512, 301], [300, 17]):
+        if form == "ragged":  # the second request's rows: the last of its length
+            m = min(n[1], rows)
+            at["cu_seqlens"].copy_(torch.tensor([0, rows, rows + m]))
+            at["prefix_lens"].copy_(torch.tensor([n[0] - rows, n[1] - m]))
+        else:
+            at["seq_lens"].copy_(torch.tensor(n))
+        ws.fill_(255)
+        g.replay()
+        assert (ws[:4] == 0).all()
+        want = run()
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("R", [8191, 8192, 8193, 20000])
+def test_pages_of_many_rows(cuda, R):
+    """Claims of table rows on chip and, past 8192 rows, in memory; rows named
+    more than once."""
+    rng = np.random.default_rng(72)
+    P, W, BS, n = 6000, 3, 16, 1700
+    lens = np.where(rng.random(R) < 0.1, rng.integers(1, 2 * BS, R), 0).astype(np.int32)
+    table, refs, free = np.full((R, W), -1, np.int32), np.zeros(P, np.int32), list(rng.permutation(P))
+    for r in np.nonzero(lens)[0]:
+        for b in range(-(-int(lens[r]) // BS)):
+            table[r, b] = free.pop()
+            refs[table[r, b]] = 1
+    data = [rng.integers(0, 1 << 30, (P, 4)).astype(np.int32)]
+    pool = O8.Pool(table, lens, refs, BS, data)
+    i32 = lambda x: torch.tensor(np.asarray(x, np.int32), device=cuda)  # noqa: E731
+    bt, sl, rf, t = i32(table), i32(lens), i32(refs), [torch.from_numpy(data[0].copy()).to(cuda)]
+    full = np.nonzero(lens)[0]
+    par, kid = rng.choice(full, n), rng.integers(R - 900, R, n)  # children named twice on average
+    short = ops.pages_fork(i32(par), i32(kid), bt, sl, rf, t, block_size=BS)
+    assert int(short) == pool.fork(par, kid)
+    rows = rng.integers(0, R, n)
+    rows[::3] = R - 1 - rng.integers(0, 40, len(rows[::3]))
+    new = pool.lens[rows] + rng.integers(0, 30, n)
+    short = ops.pages_extend(i32(rows), i32(new), bt, sl, rf, block_size=BS)
+    assert int(short) == pool.extend(rows, new)
+    for got, want in ((bt, pool.table), (sl, pool.lens), (rf, pool.refs), (t[0], pool.data[0])):
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
