@@ -756,7 +756,8 @@ typedef struct {
  * V apart: s = the smallest power of two with max|x| <= qmax * s over the finite
  * new elements (qmax 448 for e4m3, 127 for int8; s >= 2^-64); a page that holds
  * earlier tokens keeps the larger of that and its scale, and if it grew the
- * earlier codes become round(code * old / s).  New codes are round(x / s), to
+ * earlier codes become round(code * old / s).  New codes are round(x / s) (both
+ * from fp32 quotients: exact unless another writer's scale is no power of two), to
  * nearest even and saturated (infinities to the largest code; NaN stays NaN in
  * e4m3 and is 0 in int8).  A page whose first token is new starts afresh: its
  * old scale is not read.  No page may be shared by two requests of the call. */
@@ -773,12 +774,17 @@ SRSWA_API int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, con
  * sm_scale * q . k + bias over them (in fp32 log2 units: a finite bias beyond
  * +-2.35e38 counts as that; keys with one of -inf weigh 0); out [N, H, D]
  * (out_dtype: q's type or F32) and lse_out [N, H] fp32 natural log (optional).
- * A row that sees nothing, or no key of any weight, gives 0 and -inf.  Codes of keys that a row does not see never reach its
- * result, whatever they hold; NaN in those that it sees does.  workspace:
- * srswa_cache8_attend_workspace_size bytes, 16-byte aligned (0: none).  Calls
- * with many rows per request go to tensor-core tiles: their workspace is 16
- * bytes, whose first 4 are the call's status word (srswa_workspace_status); of
- * the others it is scratch. */
+ * A row that sees nothing, or no key of any weight, gives 0 and -inf.  Codes of
+ * keys that a row does not see never reach its result, whatever they hold, nor do
+ * the scales of pages that it does not see; NaN in those that it sees does.
+ * Against 64 bits, with softmax weights p (held in f16) and value scales s: out is
+ * within its type's rounding and 2^-10 sum p |v|, and each key may be off by
+ * another 2^-32 max(p s) |code|; results under 2^-126 may be 0; lse is within
+ * (D + 2) 2^-24 of the row's largest sum |q k| sm_scale.
+ * workspace: srswa_cache8_attend_workspace_size bytes, 16-byte aligned (0: none).
+ * Calls with many rows per request go to tensor-core tiles: their workspace is 16
+ * bytes, whose first 4 are the call's status word (srswa_workspace_status); of the
+ * others it is scratch. */
 SRSWA_API size_t srswa_cache8_attend_workspace_size(const srswa_cache8_desc* d, int varlen);
 SRSWA_API int srswa_cache8_attend(const srswa_cache8_desc* d, const void* q, const void* k_cache,
                                   const void* v_cache, const float* k_scale, const float* v_scale,

@@ -32,9 +32,9 @@
 // streams its units through a private cp.async ring; page ids, scales and biases
 // are prefetched a block of 32 slots ahead.
 //
-// Measured: six requests of 30k to 131k keys, 32 / 8 heads of 128 (750 MB) 134.5
-// us, 86 % of the copy rate; 256 requests with a window of 512 and 8 selected
-// pages (672 MB) 126 us, 83 %.  A unit of 32 keys takes a warp about 1.3 us from
+// Measured: six requests of 30k to 131k keys, 32 / 8 heads of 128 (750 MB) 134
+// us, 87 % of the copy rate; 256 requests with a window of 512 and 8 selected
+// pages (672 MB) 126 us, 82 %.  A unit of 32 keys takes a warp about 1.3 us from
 // one dependent step to the next, so few short items are bound by that chain:
 // 16 requests of 1024 keys 12.2 us.
 
@@ -747,8 +747,10 @@ RowsPlan rows_plan(const srswa_cache8_desc& d, bool varlen) {
     //   128  12.1  14.5  15.3   17.2  17.3  20.8   27.9  23.0  25.0   50.7  38.0  38.4   91.6  59.0  59.4
     //   256  12.6  26.8  23.7   18.2  32.5  29.4   31.9  50.2  41.9   53.2  71.8  63.0   95.6 108.2 101.3
     //  1024  54.3 104.2  71.2   77.1 129.0  96.8  114.6 168.9 131.5  192.6 241.0 196.1  347.6 390.3 349.4
-    // (pages in L2 up to 128 MB).  Over 13 x 8 sizes of 16 / 4 and 10 / 10 heads the
-    // rules below take 1.5 % more than the best of the three.
+    // (pages in L2 up to 128 MB).  Over 13 x 8 sizes of 16 / 4 and 10 / 10 heads,
+    // with tables as wide as the longest request, the rules below take 1.5 % more
+    // than the best of the three.  The host knows a table's width, not the lengths: a
+    // short request in a wide table takes equal parts (n = 1, L = 256: 12.9 for 7.6).
     // A join of parts costs about 6 us; a warp or a CTA per item leaves the long
     // items' ends alone on the GPU, so neither takes items of many units.
     const bool many = p.items > wave && most * slots <= 20 * p.items;  // one warp each while the others have items too

@@ -34,12 +34,15 @@
 // (The next S overwrites W behind the product that reads it: one thread issues
 // both, and its MMAs execute in order.)
 //
-// Measured: 8192 rows of 16 / 4 heads of 128 after 8192 tokens 1040 us, 790
-// TFLOP/s, 47 % of the measured bf16 rate.  A step takes 4700 cycles where its
-// MMAs take 2048: the softmax of a tile takes 3300 (its exp2 share the unit with
-// the other tile's), and the steps of the two tiles do not interleave fully.
-// Ragged prompts with a window of 512 and 64 sinks, 10 heads: 86 us, three waves
-// of CTAs that each spend about 9 us on their first codes and their output.
+// Measured: 8192 rows of 16 / 4 heads of 128 after 8192 tokens 1025 us, 803
+// TFLOP/s, 48 % of the measured bf16 rate.  Clocks inside an earlier form of 1040
+// us: a step takes 4700 cycles where its MMAs take 2048, the softmax of a tile 3300
+// (its exp2 share the unit with the other tile's); the steps of the two tiles do
+// not interleave fully.  One CTA an SM, 256 rows each: 28 us for 3 steps that are
+// all seen in part, 38 for 6 (a window of 512), 49 / 75 / 126 for 10 / 18 / 34, so
+// 20 us for the start, the end and the masked steps and 3 a step.  Ragged prompts
+// with a window of 512 and 64 sinks, 10 heads: 84 us, 220 CTAs in two rounds, the
+// second half full (as many equal ones: 38 and 30 us).
 //
 // Codes that a row does not see must not reach it: masked scores are replaced
 // before use, weights of masked keys are 0, and because 0 * NaN is not, steps
@@ -720,7 +723,9 @@ static int64_t tile_pairs(int64_t N, int64_t R, int64_t rows_per_req, int64_t G,
 // keys, for each wave of CTAs; the rows 10 and 1.6 per unit of 32 keys that a
 // resident warp has.  (16 / 4 heads of 128, rows and tiles: 16 rows after 4096 keys
 // 33 and 98, 32 requests of them 196 and 105; 300 such ragged rows in 4 requests
-// 166 and 112.  Over 585 sizes the choice takes 2 % more than the better one.)
+// 166 and 112.  Over 585 sizes, all with tables as wide as the longest request, the
+// choice takes 2 % more than the better one; the width stands for the lengths,
+// which the host does not know.)
 bool prompt_applies(const srswa_cache8_desc& d, bool varlen) {
   const int64_t G = d.H / d.Hkv;
   if (d.K > 0 || G > 128 || d.nsplit > 0) return false;
