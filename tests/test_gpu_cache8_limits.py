@@ -440,3 +440,20 @@ def test_pages_of_many_rows(cuda, R):
     assert int(short) == pool.extend(rows, new)
     for got, want in ((bt, pool.table), (sl, pool.lens), (rf, pool.refs), (t[0], pool.data[0])):
         np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 400])
+@pytest.mark.parametrize("W,P", [(0, 0), (0, 5), (3, 0)])
+def test_empty_tables_and_pools(cuda, rows, W, P):
+    """A table of no blocks, a cache of no pages: nothing is written or seen."""
+    R, H, Hkv, D, BS = 2, 4, 2, 128, 64
+    c = cache8.Cache8(P, BS, Hkv, D, device=cuda)
+    bt = torch.zeros(R, W, dtype=torch.int32, device=cuda)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.randn(R * rows, H, D, device=cuda).to(torch.bfloat16)
+    before = c.k.view(torch.uint8).clone()
+    for at in (dict(seq_lens=i32([0, rows])), dict(cu_seqlens=i32([0, rows, 2 * rows]), prefix_lens=i32([0, 7]))):
+        c.append(q[:, :Hkv], q[:, :Hkv], bt, **at)
+        o, lse = c.attend(q, bt, lse=True, **at)
+        assert (o == 0).all() and torch.isneginf(lse).all()
+    assert torch.equal(before, c.k.view(torch.uint8))

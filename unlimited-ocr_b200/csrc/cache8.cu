@@ -331,6 +331,12 @@ static int check_common(const srswa_cache8_desc* d, const int32_t* seq_lens, con
   return SRSWA_OK;
 }
 
+// A pool of no pages and a table of no blocks have no addresses.
+static bool there(const srswa_cache8_desc* d, const void* k, const void* v, const void* ks, const void* vs,
+                  const void* table) {
+  return (d->P == 0 || (k && v && ks && vs)) && (d->W == 0 || table);
+}
+
 static RowMap row_map(const srswa_cache8_desc* d, const int32_t* seq_lens, const int32_t* cu_rows,
                       const int32_t* prefix_lens) {
   return RowMap{seq_lens, cu_rows, prefix_lens, d->R, d->rows_per_req};
@@ -345,7 +351,7 @@ extern "C" int srswa_cache8_append(const srswa_cache8_desc* d, const void* k, co
   if (rc) return rc;
   SRSWA_CHECK_ARG(d->q_dtype == SRSWA_F32 || d->q_dtype == SRSWA_BF16 || d->q_dtype == SRSWA_F16, SRSWA_EUNSUPPORTED);
   if (d->N == 0) return SRSWA_OK;
-  SRSWA_CHECK_ARG(k && v && k_cache && v_cache && k_scale && v_scale && block_table, SRSWA_EINVAL);
+  SRSWA_CHECK_ARG(k && v && there(d, k_cache, v_cache, k_scale, v_scale, block_table), SRSWA_EINVAL);
   SRSWA_CHECK_ARG(aligned(k, 16) && aligned(v, 16) && aligned(k_cache, 16) && aligned(v_cache, 16), SRSWA_EALIGN);
   const int64_t m = d->q_dtype == SRSWA_F32 ? 3 : 7;
   SRSWA_CHECK_ARG(((d->s_qn | d->s_qh | d->s_on | d->s_oh) & m) == 0, SRSWA_EALIGN);
@@ -399,7 +405,7 @@ extern "C" int srswa_cache8_attend(const srswa_cache8_desc* desc, const void* q,
   SRSWA_CHECK_ARG(d->out_dtype == d->q_dtype || d->out_dtype == SRSWA_F32, SRSWA_EUNSUPPORTED);
   SRSWA_CHECK_ARG(d->H <= 65535 && d->N < (1ll << 31) && d->K <= kMaxSelected, SRSWA_ETOOLARGE);
   if (d->N == 0) return SRSWA_OK;
-  SRSWA_CHECK_ARG(q && k_cache && v_cache && k_scale && v_scale && block_table && out, SRSWA_EINVAL);
+  SRSWA_CHECK_ARG(q && there(d, k_cache, v_cache, k_scale, v_scale, block_table) && out, SRSWA_EINVAL);
   SRSWA_CHECK_ARG(d->K == 0 || topk_idx, SRSWA_EINVAL);
   SRSWA_CHECK_ARG(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16), SRSWA_EALIGN);
   SRSWA_CHECK_ARG(((d->s_qn | d->s_qh | d->s_on | d->s_oh) & 7) == 0, SRSWA_EALIGN);
